@@ -452,6 +452,10 @@ lcError_t lcVitBlockSessionDestroy(lcVitBlockSession* s);
 /* Uploads (and converts) the weights; they stay resident. */
 lcError_t lcVitBlockSessionSetWeights(lcVitBlockSession* s, const float* w_conv, const float* w_qkv,
                                       const float* w_o);
+/* A layer norm of the tokens over `embed` before the QKV projection, with
+ * weight and bias [embed] (uploaded, resident); both NULL: no norm, as at
+ * creation. */
+lcError_t lcVitBlockSessionSetNorm(lcVitBlockSession* s, const float* weight, const float* bias, float eps);
 /* One forward: x uploaded when non-NULL (else the resident input is reused),
  * out downloaded when non-NULL; synchronises when out is non-NULL. */
 lcError_t lcVitBlockSessionForward(lcVitBlockSession* s, const float* x, float* out);
@@ -460,6 +464,139 @@ lcError_t lcVitBlockSessionRunCached(lcVitBlockSession* s, size_t repeat_count);
 
 lcError_t lcVitBlockForward(const float* x, const float* w_conv, const float* w_qkv, const float* w_o, float* out,
                             const lcVitBlockConfig* cfg, lcDeviceKind device);
+
+/* --- operators of a decoder that reads an encoder's states -------------------
+ * New surface (the reference has self attention on host arrays only).  These
+ * calls take the caller's tensors in device memory of the library's device and
+ * launch on the caller's stream; they allocate nothing, synchronise nothing and
+ * may be captured into a graph.  What they need beside their tensors is a
+ * workspace of the caller's (its size is a function of the shape; 16-byte
+ * aligned; in use until the call's work on the stream is done).  Calls that
+ * overlap on different streams, and graphs that may run at once, need
+ * workspaces of their own.  Outputs must not overlap inputs or each other.
+ * Arguments are checked before any launch; what only the device knows (lengths,
+ * page numbers) is held to its bounds there. */
+
+/* A hipStream_t; NULL is HIP's default stream. */
+typedef void* lcStream;
+/* The library's own stream, on which the calls on host arrays run. */
+lcError_t lcHipBackendStream(lcStream* out);
+
+/* A [batch, heads, rows, d] tensor; d is contiguous, the strides count
+ * elements and are not negative.  An input's may be zero (broadcast). */
+typedef struct lcDeviceTensor {
+  void* data;
+  int64_t stride_batch;
+  int64_t stride_head;
+  int64_t stride_row;
+} lcDeviceTensor;
+
+/* Cross attention: out = softmax(scale q k^T) v over the first kv_lengths[b]
+ * keys of batch row b (all kv_len when kv_lengths is NULL; values outside
+ * [0, kv_len] are held to it).  Query head h reads key/value head
+ * h / (heads / kv_heads).  q, out [batch, heads, q_len, head_dim];
+ * k, v [batch, kv_heads, kv_len, head_dim], all in dtype; lse (may be NULL)
+ * [batch, heads, q_len] fp32 contiguous: the log of each row's sum of
+ * exponentials.  A row without keys gives zeros and lse = -inf.  Keys and values
+ * past a row's length are not read.  head_dim <= 128 (else LC_NOT_SUPPORTED);
+ * q_len, kv_len and batch may be 0; scale 0 means 1 / sqrt(head_dim).
+ * Sums, the softmax and products accumulate in fp32; with 16-bit types the
+ * probabilities are rounded to that type for the second product. */
+typedef struct lcCrossAttentionConfig {
+  size_t batch;
+  size_t heads;
+  size_t kv_heads;
+  size_t q_len;
+  size_t kv_len;
+  size_t head_dim;
+  lcDataType dtype;
+  float scale;
+} lcCrossAttentionConfig;
+
+lcError_t lcCrossAttentionWorkspaceSize(const lcCrossAttentionConfig* cfg, int backward, size_t* bytes);
+lcError_t lcCrossAttentionForward(const lcCrossAttentionConfig* cfg, const lcDeviceTensor* q, const lcDeviceTensor* k,
+                                  const lcDeviceTensor* v, const int32_t* kv_lengths, const lcDeviceTensor* out,
+                                  float* lse, void* workspace, size_t workspace_bytes, lcStream stream);
+/* Gradients of the forward with the same cfg and kv_lengths; out and lse are
+ * its results.  dq like q; dk, dv like k, v (summed over the query heads that
+ * share a head; zero past a row's length).  Every gradient is written by one
+ * workgroup or summed in a fixed order: equal calls give equal bits. */
+lcError_t lcCrossAttentionBackward(const lcCrossAttentionConfig* cfg, const lcDeviceTensor* dout,
+                                   const lcDeviceTensor* q, const lcDeviceTensor* k, const lcDeviceTensor* v,
+                                   const lcDeviceTensor* out, const float* lse, const int32_t* kv_lengths,
+                                   const lcDeviceTensor* dq, const lcDeviceTensor* dk, const lcDeviceTensor* dv,
+                                   void* workspace, size_t workspace_bytes, lcStream stream);
+
+/* Layer norm of `rows` rows of n values (row strides in elements):
+ * y = (x - mean) rstd weight + bias, rstd = 1 / sqrt(var + eps), var the mean
+ * squared deviation.  x, y in dtype; weight, bias [n] in weight_dtype (dtype or
+ * f32), NULL for 1 and 0; mean, rstd [rows] fp32, both or neither.  y may be x
+ * itself. */
+typedef struct lcLayerNormConfig {
+  size_t rows;
+  size_t n;
+  lcDataType dtype;
+  lcDataType weight_dtype;
+  float eps;
+} lcLayerNormConfig;
+
+lcError_t lcLayerNormForward(const lcLayerNormConfig* cfg, const void* x, int64_t x_stride, const void* weight,
+                             const void* bias, void* y, int64_t y_stride, float* mean, float* rstd, lcStream stream);
+/* Gradients: dx [rows, n] in dtype; dweight, dbias [n] in weight_dtype, summed
+ * over the rows in fp32 in a fixed order (either may be NULL).  weight NULL
+ * means 1.  The workspace is the backward pass's. */
+lcError_t lcLayerNormWorkspaceSize(const lcLayerNormConfig* cfg, size_t* bytes);
+lcError_t lcLayerNormBackward(const lcLayerNormConfig* cfg, const void* dy, int64_t dy_stride, const void* x,
+                              int64_t x_stride, const void* weight, const float* mean, const float* rstd, void* dx,
+                              int64_t dx_stride, void* dweight, void* dbias, void* workspace, size_t workspace_bytes,
+                              lcStream stream);
+
+/* An 8-bit cache of keys and values in pages of 64 tokens.  k_pages
+ * [pages, kv_heads, 64, head_dim] and v_pages [pages, kv_heads, head_dim, 64]
+ * hold e4m3 codes (OCP, no infinities), k_scales and v_scales
+ * [pages, kv_heads] what a code of 1 stands for; all contiguous, pages 16-byte
+ * aligned.  head_dim a multiple of 16, at most 128.  block_table
+ * [batch, table_width] (row stride table_stride) names the pages of each
+ * sequence in order; entries past its length are not read. */
+typedef struct lcKvCache {
+  void* k_pages;
+  void* v_pages;
+  float* k_scales;
+  float* v_scales;
+  size_t pages;
+  size_t kv_heads;
+  size_t head_dim;
+} lcKvCache;
+
+/* Writes the first kv_lengths[b] (NULL: kv_len) tokens of k, v
+ * [batch, kv_heads, kv_len, head_dim] to row b's pages, from their start: scale
+ * = max(amax / 448, 2^-126) over a page of one head, code = e4m3(x / scale) to
+ * the nearest, ties to even; the rest of a last page becomes zeros.  A page
+ * outside the pool is not written; pages that no row names stay as they are.
+ * Rows that name one page must bring the same tokens for it. */
+lcError_t lcKvCacheStore(const lcKvCache* cache, size_t batch, size_t kv_len, lcDataType dtype,
+                         const lcDeviceTensor* k, const lcDeviceTensor* v, const int32_t* block_table,
+                         size_t table_width, int64_t table_stride, const int32_t* kv_lengths, lcStream stream);
+
+/* Attention of q [batch, heads, q_len, head_dim] over the first kv_lengths[b]
+ * (NULL: 64 table_width; more is held to that) tokens of row b's pages, as
+ * lcCrossAttentionForward.  Made for few query rows: each block of 16 rows that
+ * share a head reads the head's pages once.  A page outside the pool is not
+ * read; the rows that would need it come out as NaN. */
+typedef struct lcKvAttentionConfig {
+  size_t batch;
+  size_t heads;
+  size_t q_len;
+  size_t table_width;
+  lcDataType dtype;
+  float scale;
+} lcKvAttentionConfig;
+
+lcError_t lcKvCacheAttentionWorkspaceSize(const lcKvCache* cache, const lcKvAttentionConfig* cfg, size_t* bytes);
+lcError_t lcKvCacheAttention(const lcKvCache* cache, const lcKvAttentionConfig* cfg, const lcDeviceTensor* q,
+                             const int32_t* block_table, int64_t table_stride, const int32_t* kv_lengths,
+                             const lcDeviceTensor* out, float* lse, void* workspace, size_t workspace_bytes,
+                             lcStream stream);
 
 /* --- device info and timing on the backend stream ---------------------------- */
 

@@ -17,6 +17,7 @@
 //    transposed V); attention, writing heads concatenated [B*T, E]; the output
 //    projection.  CJ_HIP_VIT_PATCHIFY=0 selects the implicit-im2col GEMM.
 #include <algorithm>
+#include <cmath>
 #include <cstdlib>
 #include <cstring>
 #include <map>
@@ -281,6 +282,10 @@ struct lcVitBlockSession {
   // vitPatchify layout and the patch conv is a row-major GEMM), else as
   // 16-bit NCHW read by the implicit-im2col GEMM.
   bool patchify = false;
+  // The norm before the QKV projection: weight, then bias, fp32 [embed] each.
+  DeviceBuffer norm;
+  bool has_norm = false;
+  float norm_eps = 0.0f;
 };
 
 namespace {
@@ -331,6 +336,24 @@ Status vitForwardDevice(HipContext* ctx, lcVitBlockSession* s) {
                                             static_cast<int>(c.patch), E, ht, ctx->stream);
   if (e != hipSuccess) {
     return failHip(e, "vit patch-embed launch");
+  }
+  if (s->has_norm) {
+    // In place: each row is read whole before it is written.
+    kern::LayerNormArgs ln{};
+    ln.x = s->tokens16.get();
+    ln.y = s->tokens16.get();
+    ln.w = s->norm.as<float>();
+    ln.b = s->norm.as<float>() + c.embed;
+    ln.rows = M;
+    ln.n = E;
+    ln.sx = ln.sy = E;
+    ln.wide = 1;
+    ln.eps = s->norm_eps;
+    e = kern::layerNorm(ln, c.compute_dtype == LC_DTYPE_F16 ? kern::DType::kF16 : kern::DType::kBF16, false, true,
+                        ctx->stream);
+    if (e != hipSuccess) {
+      return failHip(e, "vit norm launch");
+    }
   }
   traceOpDispatch(TraceOp::kMatMul, Device::kHIP, Device::kHIP, false, s->M * c.embed * 3 * c.embed);
   e = kern::qkvProjectGemm(s->tokens16.as<uint16_t>(), s->wqkv_t16.as<uint16_t>(), s->q16.as<uint16_t>(),
@@ -748,6 +771,34 @@ lcError_t lcVitBlockSessionSetWeights(lcVitBlockSession* s, const float* w_conv,
   if (st == Status::kSuccess) {
     s->has_w = true;
   }
+  return toLc(st);
+}
+
+lcError_t lcVitBlockSessionSetNorm(lcVitBlockSession* s, const float* weight, const float* bias, float eps) {
+  if (s == nullptr || (weight == nullptr) != (bias == nullptr)) {
+    return toLc(fail(Status::kInvalidValue, "vit block: null session, or a norm's weight without its bias"));
+  }
+  if (!std::isfinite(eps) || eps < 0.0f) {
+    return toLc(fail(Status::kInvalidValue, "vit block: the norm's eps must be finite and not negative"));
+  }
+  HipContext* ctx = nullptr;
+  Status st = requireHip(s->device, "vit block", &ctx);
+  if (st != Status::kSuccess) {
+    return toLc(st);
+  }
+  std::lock_guard<std::recursive_mutex> lock(ctx->mu);
+  if (weight == nullptr) {
+    s->has_norm = false;
+    return LC_SUCCESS;
+  }
+  const std::size_t n = s->cfg.embed;
+  st = s->norm.ensure(2 * n * sizeof(float));
+  if (st == Status::kSuccess) st = upload(ctx, s->norm.get(), weight, n * sizeof(float));
+  if (st == Status::kSuccess) st = upload(ctx, s->norm.as<float>() + n, bias, n * sizeof(float));
+  if (st == Status::kSuccess) st = syncStream(ctx);
+  // A failure leaves the block without a norm rather than with half of one.
+  s->has_norm = st == Status::kSuccess;
+  s->norm_eps = eps;
   return toLc(st);
 }
 

@@ -333,4 +333,108 @@ hipError_t attentionHalf(const uint16_t* q, const uint16_t* k, const uint16_t* v
                          uint16_t* out_heads_concat, int heads, int bh, int S, int S_pad, int D, bool causal, Half t,
                          int cus, hipStream_t stream);
 
+// ---- cross attention (cross_attention.hip) -----------------------------------
+enum class DType { kF32, kBF16, kF16 };
+// A [batch, heads, rows, d] tensor on the device, d contiguous; strides in
+// elements.
+struct XTensor {
+  void* p = nullptr;
+  int64_t sb = 0;
+  int64_t sh = 0;
+  int64_t ss = 0;
+};
+struct XAttnArgs {
+  XTensor q, k, v, o, go, dq, dk, dv;  // backward: o and go (dO) are read
+  float* lse;                          // [batch, heads, q_len]; the forward's may be null
+  float* delta;                        // backward: [batch, heads, q_len][2]
+  const int32_t* lengths;              // [batch] keys of each batch row, or null (all kv_len)
+  int batch, heads, kv_heads, q_len, kv_len, d;
+  float c;      // |scale| * log2(e); `negate` when scale < 0
+  float scale;
+  int negate;
+  int splits;    // workgroups that share a row block's tiles
+  float* part;   // splits > 1: [splits][rows][kXAttnWidth(d)]
+  float* stats;  // splits > 1, forward: [splits][rows][2]
+};
+constexpr int kXAttnRows = 128;  // rows (or keys) of a workgroup
+constexpr int kXAttnMaxDim = 128;
+constexpr int kXAttnWidth(int d) { return d <= 64 ? 64 : 128; }
+constexpr int kXAttnTile(DType t) { return t == DType::kF32 ? 32 : 64; }
+enum class XAttnStep { kForward, kGradQ, kGradKV };
+// One kernel of the set.  `aligned`: every tensor's base is 16-byte aligned, its
+// strides and d are multiples of 16 bytes.
+hipError_t crossAttention(XAttnStep step, const XAttnArgs& a, DType type, bool aligned, hipStream_t stream);
+// Joins the forward's splits; sums the backward's (x, then `second`, each
+// [batch, heads, len, d], from part [splits][1 or 2][batch * heads * len][width]).
+hipError_t crossAttentionJoin(const XAttnArgs& a, DType type, hipStream_t stream);
+hipError_t crossAttentionSum(const float* part, const XTensor& x, const XTensor* second, int splits, int batch,
+                             int heads, int len, int d, DType type, hipStream_t stream);
+
+// ---- layer norm (layer_norm.hip) ----------------------------------------------
+// Rows of n values with row strides in elements.  Forward: x -> y (mean and
+// rstd stored when not null).  Backward: x, dy (stride sy), mean, rstd -> dx,
+// and dw / db (either may be null) by way of part
+// [layerNormGroups(rows, n, true, chunk)][2][n].
+struct LayerNormArgs {
+  const void* x;
+  const void* dy;
+  void* y;
+  void* dx;
+  const void* w;
+  const void* b;
+  void* dw;
+  void* db;
+  float* mean;
+  float* rstd;
+  float* part;
+  int64_t rows;
+  int64_t sx, sy, sdx;
+  int n;
+  int wide;  // w, b, dw and db are fp32 (else x's type)
+  float eps;
+};
+// chunk: values of x in 16 bytes.
+int layerNormLanes(int64_t rows, int n, int chunk);
+int layerNormGroups(int64_t rows, int n, bool backward, int chunk);
+hipError_t layerNorm(const LayerNormArgs& a, DType type, bool backward, bool aligned, hipStream_t stream);
+
+// ---- 8-bit paged key/value cache (kv_cache.hip) --------------------------------
+constexpr int kKvPage = 64;  // tokens of a page
+// k, v [batch, heads, kv_len, d] -> the pages that row b's table names, up to
+// its length; d a multiple of 16, at most 128.  `aligned`: 16-byte bases and
+// strides.
+struct KvStoreArgs {
+  XTensor k, v;
+  const int32_t* lengths;
+  const int32_t* table;
+  int64_t table_stride;
+  uint8_t* k_pages;  // [pages, heads, 64, d]
+  uint8_t* v_pages;  // [pages, heads, d, 64]
+  float* k_scales;   // [pages, heads]
+  float* v_scales;
+  int batch, heads, kv_len, d, pages;
+};
+hipError_t kvStore(const KvStoreArgs& a, DType type, bool aligned, hipStream_t stream);
+// q, o [batch, heads, q_len, d]; row b attends to the first lengths[b] tokens of
+// its table's pages (at most kv_len = 64 * the table's width).  splits > 1:
+// part and stats as for crossAttentionJoin.
+struct KvAttnArgs {
+  XTensor q, o;
+  float* lse;
+  const int32_t* lengths;
+  const int32_t* table;
+  int64_t table_stride;
+  const uint8_t* k_pages;
+  const uint8_t* v_pages;
+  const float* k_scales;
+  const float* v_scales;
+  int batch, heads, kv_heads, q_len, kv_len, d, pages;
+  float c;  // scale * log2(e)
+  int aligned;  // q: 16-byte base and strides
+  int splits;
+  float* part;
+  float* stats;
+};
+hipError_t kvAttention(const KvAttnArgs& a, DType type, hipStream_t stream);
+
 }  // namespace lchip::kern

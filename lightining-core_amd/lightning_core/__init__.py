@@ -8,6 +8,8 @@ bind_integrated.cpp): same function names, argument names and error behaviour
 
 * the default device is "hip" (the only device this library computes on);
   "cpu", "cuda" and "metal" are accepted and answer "not supported";
+* cross attention, layer norm and an 8-bit key/value cache (_decoder.py) are
+  additions; they take torch tensors in GPU memory as well as numpy arrays;
 * half-precision compute is an explicit `compute_dtype` argument on the new
   batched-attention, resident-matmul and ViT-block entry points.
 
@@ -18,6 +20,8 @@ from ._core import *  # noqa: F401,F403
 from ._core import __all__ as _core_all
 from ._graph import *  # noqa: F401,F403
 from ._graph import __all__ as _graph_all
+from ._decoder import *  # noqa: F401,F403
+from ._decoder import __all__ as _decoder_all
 from . import api  # noqa: F401
 
-__all__ = list(_core_all) + list(_graph_all)
+__all__ = list(_core_all) + list(_graph_all) + list(_decoder_all)

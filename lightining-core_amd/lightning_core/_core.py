@@ -742,6 +742,18 @@ class VitBlockSession:
             raise ValueError("weight shape mismatch")
         _check(_lib().lcVitBlockSessionSetWeights(self._h, _fp(w_conv), _fp(w_qkv), _fp(w_o)))
 
+    def set_norm(self, weight, bias=None, eps=1e-5):
+        """A layer norm of the tokens before the QKV projection; weight None
+        takes it out again."""
+        if weight is None:
+            _check(_lib().lcVitBlockSessionSetNorm(self._h, None, None, eps))
+            return
+        weight = _f32(weight)
+        bias = np.zeros_like(weight) if bias is None else _f32(bias)
+        if weight.shape != (self.cfg.embed,) or bias.shape != (self.cfg.embed,):
+            raise ValueError("weight and bias must hold embed values")
+        _check(_lib().lcVitBlockSessionSetNorm(self._h, _fp(weight), _fp(bias), eps))
+
     def forward(self, x=None, download=True):
         xa = None
         if x is not None:

@@ -116,6 +116,31 @@ class GraphPlannerOptions(ctypes.Structure):
                 ("planner_cost_weight_preference", ctypes.c_double)]
 
 
+class DeviceTensor(ctypes.Structure):
+    """lcDeviceTensor."""
+    _fields_ = [("data", c_void_p), ("stride_batch", ctypes.c_int64), ("stride_head", ctypes.c_int64),
+                ("stride_row", ctypes.c_int64)]
+
+
+class CrossAttentionConfig(ctypes.Structure):
+    _fields_ = [("batch", c_size), ("heads", c_size), ("kv_heads", c_size), ("q_len", c_size), ("kv_len", c_size),
+                ("head_dim", c_size), ("dtype", c_int), ("scale", c_float)]
+
+
+class LayerNormConfig(ctypes.Structure):
+    _fields_ = [("rows", c_size), ("n", c_size), ("dtype", c_int), ("weight_dtype", c_int), ("eps", c_float)]
+
+
+class KvCache(ctypes.Structure):
+    _fields_ = [("k_pages", c_void_p), ("v_pages", c_void_p), ("k_scales", c_void_p), ("v_scales", c_void_p),
+                ("pages", c_size), ("kv_heads", c_size), ("head_dim", c_size)]
+
+
+class KvAttentionConfig(ctypes.Structure):
+    _fields_ = [("batch", c_size), ("heads", c_size), ("q_len", c_size), ("table_width", c_size), ("dtype", c_int),
+                ("scale", c_float)]
+
+
 class HipDeviceInfo(ctypes.Structure):
     _fields_ = [("name", ctypes.c_char * 128), ("gcn_arch", ctypes.c_char * 64), ("compute_units", c_int),
                 ("max_clock_khz", c_int), ("total_memory_bytes", c_size), ("l2_cache_bytes", c_size)]
@@ -208,9 +233,26 @@ SIGNATURES = {
     "lcVitBlockSessionCreate": (_E, [P(VitBlockConfig), c_int, P(c_void_p)]),
     "lcVitBlockSessionDestroy": (_E, [c_void_p]),
     "lcVitBlockSessionSetWeights": (_E, [c_void_p, BUF, BUF, BUF]),
+    "lcVitBlockSessionSetNorm": (_E, [c_void_p, BUF, BUF, c_float]),
     "lcVitBlockSessionForward": (_E, [c_void_p, BUF, BUF]),
     "lcVitBlockSessionRunCached": (_E, [c_void_p, c_size]),
     "lcVitBlockForward": (_E, [BUF, BUF, BUF, BUF, BUF, P(VitBlockConfig), c_int]),
+    "lcHipBackendStream": (_E, [P(c_void_p)]),
+    "lcCrossAttentionWorkspaceSize": (_E, [P(CrossAttentionConfig), c_int, P(c_size)]),
+    "lcCrossAttentionForward": (_E, [P(CrossAttentionConfig)] + [P(DeviceTensor)] * 3 + [BUF, P(DeviceTensor), BUF, BUF,
+                                                                                       c_size, c_void_p]),
+    "lcCrossAttentionBackward": (_E, [P(CrossAttentionConfig)] + [P(DeviceTensor)] * 5 + [BUF, BUF]
+                                 + [P(DeviceTensor)] * 3 + [BUF, c_size, c_void_p]),
+    "lcLayerNormWorkspaceSize": (_E, [P(LayerNormConfig), P(c_size)]),
+    "lcLayerNormForward": (_E, [P(LayerNormConfig), BUF, ctypes.c_int64, BUF, BUF, BUF, ctypes.c_int64, BUF, BUF,
+                                c_void_p]),
+    "lcLayerNormBackward": (_E, [P(LayerNormConfig), BUF, ctypes.c_int64, BUF, ctypes.c_int64, BUF, BUF, BUF, BUF,
+                                 ctypes.c_int64, BUF, BUF, BUF, c_size, c_void_p]),
+    "lcKvCacheStore": (_E, [P(KvCache), c_size, c_size, c_int, P(DeviceTensor), P(DeviceTensor), BUF, c_size,
+                            ctypes.c_int64, BUF, c_void_p]),
+    "lcKvCacheAttentionWorkspaceSize": (_E, [P(KvCache), P(KvAttentionConfig), P(c_size)]),
+    "lcKvCacheAttention": (_E, [P(KvCache), P(KvAttentionConfig), P(DeviceTensor), BUF, ctypes.c_int64, BUF,
+                                P(DeviceTensor), BUF, BUF, c_size, c_void_p]),
     "lcHipGetDeviceInfo": (_E, [P(HipDeviceInfo)]),
     "lcHipTimerCreate": (_E, [P(c_void_p)]),
     "lcHipTimerDestroy": (_E, [c_void_p]),
