@@ -475,12 +475,17 @@ lcError_t lcVitBlockForward(const float* x, const float* w_conv, const float* w_
  * overlap on different streams, and graphs that may run at once, need
  * workspaces of their own.  Outputs must not overlap inputs or each other.
  * Arguments are checked before any launch; what only the device knows (lengths,
- * page numbers) is held to its bounds there. */
+ * page numbers) is held to its bounds there.  That a pointer is memory of the
+ * library's device is asked of HIP, 0.3 us each, unless the caller vouches for
+ * it (trusted_pointers not 0), as a binding does whose tensors know where they
+ * are; a trusted pointer that is not faults the device. */
 
 /* A hipStream_t; NULL is HIP's default stream. */
 typedef void* lcStream;
 /* The library's own stream, on which the calls on host arrays run. */
 lcError_t lcHipBackendStream(lcStream* out);
+/* The HIP ordinal of the library's device. */
+lcError_t lcHipDeviceIndex(int* out);
 
 /* A [batch, heads, rows, d] tensor; d is contiguous, the strides count
  * elements and are not negative.  An input's may be zero (broadcast). */
@@ -511,6 +516,7 @@ typedef struct lcCrossAttentionConfig {
   size_t head_dim;
   lcDataType dtype;
   float scale;
+  int trusted_pointers;
 } lcCrossAttentionConfig;
 
 lcError_t lcCrossAttentionWorkspaceSize(const lcCrossAttentionConfig* cfg, int backward, size_t* bytes);
@@ -538,6 +544,7 @@ typedef struct lcLayerNormConfig {
   lcDataType dtype;
   lcDataType weight_dtype;
   float eps;
+  int trusted_pointers;
 } lcLayerNormConfig;
 
 lcError_t lcLayerNormForward(const lcLayerNormConfig* cfg, const void* x, int64_t x_stride, const void* weight,
@@ -566,6 +573,7 @@ typedef struct lcKvCache {
   size_t pages;
   size_t kv_heads;
   size_t head_dim;
+  int trusted_pointers; /* of calls on this cache, their other tensors' too */
 } lcKvCache;
 
 /* Writes the first kv_lengths[b] (NULL: kv_len) tokens of k, v

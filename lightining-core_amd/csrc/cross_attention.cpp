@@ -13,11 +13,16 @@ constexpr std::size_t kMostRows = std::size_t{1} << 30;
 // Workgroups that fill the chip (256 CUs, two each).  A split beyond that only
 // adds partial results to join.
 constexpr std::size_t kTarget = 512;
+// Up to so many query rows of a problem, the forward's waves share the keys
+// instead of the rows (one workgroup on a CU).
+constexpr std::size_t kFewRows = 64;
+constexpr std::size_t kFewTarget = 256;
 
 // How the three kernels share the work of a problem, and the workspace that it
 // takes: a function of the shape alone, so that the size a caller asks for is
 // the one its call needs.
 struct Plan {
+  bool few = false;
   int splits_fwd = 1, splits_q = 1, splits_kv = 1;
   std::size_t rows_q = 0, rows_kv = 0;  // rows of all problems
   std::size_t width = 0;                // floats of a partial row
@@ -44,9 +49,15 @@ Plan planOf(const lcCrossAttentionConfig& c) {
   p.width = static_cast<std::size_t>(kern::kXAttnWidth(static_cast<int>(c.head_dim)));
   const std::size_t q_blocks = problems * ((group * c.q_len + block - 1) / block);
   const std::size_t kv_tiles = (c.kv_len + tile - 1) / tile;
-  p.splits_fwd = splitCount(q_blocks, kv_tiles, kTarget);
-  p.splits_q = p.splits_fwd;
-  p.splits_kv = splitCount(problems * ((c.kv_len + block - 1) / block), group * ((c.q_len + tile - 1) / tile), kTarget);
+  const std::size_t few_rows = kern::kXAttnFewRows;
+  p.few = group * c.q_len <= kFewRows;
+  p.splits_fwd = p.few ? splitCount(problems * ((group * c.q_len + few_rows - 1) / few_rows), (kv_tiles + 3) / 4,
+                                    kFewTarget)
+                       : splitCount(q_blocks, kv_tiles, kTarget);
+  p.splits_q = splitCount(q_blocks, kv_tiles, kTarget);
+  const std::size_t q_tile = kern::kXAttnQueryTile;
+  p.splits_kv = splitCount(problems * ((c.kv_len + block - 1) / block), group * ((c.q_len + q_tile - 1) / q_tile),
+                           kTarget);
   return p;
 }
 
@@ -119,7 +130,7 @@ Status forward(const lcCrossAttentionConfig* cfg, const lcDeviceTensor* q, const
   fillArgs(c, &a);
   const Plan plan = planOf(c);
   DeviceCall call;
-  LC_TRY(call.open(kOp));
+  LC_TRY(call.open(kOp, c.trusted_pointers != 0));
   if (plan.rows_q == 0) {
     return Status::kSuccess;
   }
@@ -133,6 +144,7 @@ Status forward(const lcCrossAttentionConfig* cfg, const lcDeviceTensor* q, const
   a.lse = lse;
   a.lengths = kv_lengths;
   a.splits = plan.splits_fwd;
+  a.few = plan.few ? 1 : 0;
   if (a.splits > 1) {
     LC_TRY(call.onDevice(workspace, "the workspace"));
     a.part = static_cast<float*>(workspace);
@@ -170,7 +182,7 @@ Status backward(const lcCrossAttentionConfig* cfg, const lcDeviceTensor* dout, c
     return fail(Status::kInvalidValue, "cross attention: the backward pass needs the forward's lse");
   }
   DeviceCall call;
-  LC_TRY(call.open(kOp));
+  LC_TRY(call.open(kOp, c.trusted_pointers != 0));
   LC_TRY(checkWorkspace(workspace, workspace_bytes, plan.backwardBytes()));
   const struct {
     const void* p;

@@ -11,8 +11,9 @@ DeviceCall::~DeviceCall() {
   }
 }
 
-Status DeviceCall::open(const char* op) {
+Status DeviceCall::open(const char* op, bool trusted) {
   op_ = op;
+  trusted_ = trusted;
   if (hipGetDevice(&before_) != hipSuccess) {
     (void)hipGetLastError();
     before_ = -1;
@@ -21,7 +22,7 @@ Status DeviceCall::open(const char* op) {
 }
 
 Status DeviceCall::onDevice(const void* p, const char* what) const {
-  if (p == nullptr) {
+  if (p == nullptr || trusted_) {
     return Status::kSuccess;
   }
   hipPointerAttribute_t attr{};
@@ -89,6 +90,20 @@ int splitCount(std::size_t blocks, std::size_t tiles, std::size_t target) {
 }
 
 }  // namespace lchip
+
+extern "C" lcError_t lcHipDeviceIndex(int* out) {
+  using namespace lchip;
+  if (out == nullptr) {
+    return toLc(fail(Status::kInvalidValue, "device index: null output"));
+  }
+  *out = -1;
+  DeviceCall call;
+  const Status st = call.open("device index", false);
+  if (st == Status::kSuccess) {
+    *out = call.device();
+  }
+  return toLc(st);
+}
 
 extern "C" lcError_t lcHipBackendStream(lcStream* out) {
   using namespace lchip;

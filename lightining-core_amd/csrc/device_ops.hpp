@@ -17,15 +17,17 @@ class DeviceCall {
   DeviceCall(const DeviceCall&) = delete;
   DeviceCall& operator=(const DeviceCall&) = delete;
   ~DeviceCall();
-  Status open(const char* op);
-  // kInvalidValue unless p is memory of the library's device.  Null passes: the
-  // callers have refused it where the tensor has values.
+  Status open(const char* op, bool trusted);
+  // kInvalidValue unless p is memory of the library's device (not asked where
+  // the caller vouches for its pointers).  Null passes: the callers have refused
+  // it where the tensor has values.
   Status onDevice(const void* p, const char* what) const;
   int device() const { return ctx_->device; }
 
  private:
   HipContext* ctx_ = nullptr;
   const char* op_ = "";
+  bool trusted_ = false;
   int before_ = -1;
 };
 

@@ -353,13 +353,16 @@ struct XAttnArgs {
   float scale;
   int negate;
   int splits;    // workgroups that share a row block's tiles
+  int few;       // forward: blocks of kXAttnFewRows rows, waves that share the keys
   float* part;   // splits > 1: [splits][rows][kXAttnWidth(d)]
   float* stats;  // splits > 1, forward: [splits][rows][2]
 };
 constexpr int kXAttnRows = 128;  // rows (or keys) of a workgroup
 constexpr int kXAttnMaxDim = 128;
 constexpr int kXAttnWidth(int d) { return d <= 64 ? 64 : 128; }
-constexpr int kXAttnTile(DType t) { return t == DType::kF32 ? 32 : 64; }
+constexpr int kXAttnFewRows = 32;
+constexpr int kXAttnTile(DType t) { return t == DType::kF32 ? 32 : 64; }  // keys
+constexpr int kXAttnQueryTile = 32;                                       // queries, for dK and dV
 enum class XAttnStep { kForward, kGradQ, kGradKV };
 // One kernel of the set.  `aligned`: every tensor's base is 16-byte aligned, its
 // strides and d are multiples of 16 bytes.

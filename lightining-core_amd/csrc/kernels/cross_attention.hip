@@ -139,57 +139,61 @@ __device__ __forceinline__ void pack_block(const floatx16& p, u32x4 (&pk)[2]) {
   }
 }
 
-// Two waves per SIMD, so that one computes probabilities while the other's
-// products run; wide fp32 rows and element-wise loads need the registers of one.
-template <typename T, int DP, bool VEC>
-constexpr int waves_per_simd() {
-  return DP == 128 && (Elem<T>::kChunk == 4 || !VEC) ? 1 : 2;
-}
-
-// The rows of a [rows, d] matrix with a row stride, moved tile by tile into LDS
-// through registers: 256 threads, NL chunks each.  Rows past `rows` and columns
-// past d arrive as zeros (a buffer load past its range returns zero), so no
-// address past the matrix is ever read and nothing there reaches a product.
-// The range is taken anew for each tile, so that 32-bit offsets never span more
-// than a tile.  Aligned rows (VEC) are fetched a tile ahead; others, an element
-// at a time, as they are needed.
-template <typename T, int DP, int KT, bool VEC>
+// The rows of a [rows, d] matrix with a row stride, moved into LDS tile by tile
+// by NW waves.  Rows past `rows` and columns past d arrive as zeros (a buffer
+// load past its range returns zero), so no address past the matrix is ever read
+// and nothing there reaches a product.  The range is taken anew for each tile,
+// so that 32-bit offsets never span more than a tile.  Aligned rows (VEC) are
+// copied by the LDS DMA, 1 KB an instruction: it fills LDS in lane order, so the
+// swizzle is made by choosing which chunk a lane fetches.  Other rows go through
+// registers, an element at a time.
+template <typename T, int DP, int KT, bool VEC, int NW>
 struct Stream {
   using E = typename Elem<T>::type;
   using TL = Tile<T, DP>;
-  static constexpr int NL = KT * TL::CPR / 256;
-  static constexpr int RPI = 256 / TL::CPR;  // rows between a thread's chunks
-  static_assert(NL * 256 == KT * TL::CPR, "tile");
+  static constexpr int kCopies = KT * TL::RB / 1024;  // of the whole tile
+  static constexpr int NI = kCopies / NW;             // of one wave
+  static constexpr int RPI = 64 / TL::CPR;            // rows of a copy
+  static_assert(NI * NW == kCopies, "tile");
   static constexpr int kOutside = 0x7fffffff;
-  u32x4 reg[NL];
   const E* base;
   int64_t stride;
   int rows;
   int d;
-  int row;  // this thread's first row and chunk of a tile
-  int chunk;
-  __device__ __forceinline__ void init(const void* p, int64_t stride_, int rows_, int d_, int tid) {
+  int lane;
+  int wave;
+  __device__ __forceinline__ void init(const void* p, int64_t stride_, int rows_, int d_, int wave_, int lane_) {
     base = static_cast<const E*>(p);
     stride = stride_;
     rows = rows_;
     d = d_;
-    row = tid / TL::CPR;
-    chunk = tid % TL::CPR;
+    lane = lane_;
+    wave = wave_;
   }
-  __device__ __forceinline__ void load(int tile) {
+  // Starts moving tile `tile` to lds (16-byte aligned).
+  __device__ __forceinline__ void stage(int tile, char* lds) const {
     const E* tp = base + static_cast<int64_t>(tile) * KT * stride;
     const int left = rows - tile * KT;
     const int rb = static_cast<int>(stride) * static_cast<int>(sizeof(E));
     // The last byte a tile may touch: its last row's last value.
     const int bytes = (min(left, KT) - 1) * rb + d * static_cast<int>(sizeof(E));
-    auto rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<E*>(tp), 0, bytes, 0x00027000);
+    if constexpr (VEC) {
+      const u32x4 buffer = buffer_of(tp, bytes);
+      const uint32_t to = lds_addr(lds);
 #pragma unroll
-    for (int i = 0; i < NL; ++i) {
-      const int r = row + i * RPI;
-      if constexpr (VEC) {
-        const int off = (r < left && chunk * TL::EC < d) ? r * rb + chunk * 16 : kOutside;
-        reg[i] = __builtin_amdgcn_raw_buffer_load_b128(rsrc, off, 0, 0);
-      } else {
+      for (int i = 0; i < NI; ++i) {
+        const int copy = wave + NW * i;
+        const int r = copy * RPI + lane / TL::CPR;
+        const int c = (lane % TL::CPR) ^ TL::swz(r);
+        const int off = (r < left && c * TL::EC < d) ? r * rb + c * 16 : kOutside;
+        load_lds16_buffer(static_cast<uint32_t>(off), buffer, to + static_cast<uint32_t>(copy) * 1024u);
+      }
+    } else {
+      auto rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<E*>(tp), 0, bytes, 0x00027000);
+#pragma unroll 1
+      for (int i = 0; i < NI; ++i) {
+        const int r = (wave + NW * i) * RPI + lane / TL::CPR;
+        const int chunk = lane % TL::CPR;
         u32x4 v = zero_chunk();
 #pragma unroll
         for (int e = 0; e < TL::EC; ++e) {
@@ -202,17 +206,19 @@ struct Stream {
             v[e >> 1] |= w << (16 * (e & 1));
           }
         }
-        reg[i] = v;
+        *reinterpret_cast<u32x4*>(lds + TL::at(r, chunk)) = v;
       }
     }
   }
-  __device__ __forceinline__ void store(char* lds) const {
-#pragma unroll
-    for (int i = 0; i < NL; ++i) {
-      *reinterpret_cast<u32x4*>(lds + TL::at(row + i * RPI, chunk)) = reg[i];
-    }
-  }
 };
+
+// Everything staged before has arrived, for every wave, and every wave is done
+// reading what it read before.
+__device__ __forceinline__ void arrive() {
+  wait_vmcnt<0>();
+  wait_lgkmcnt<0>();
+  stage_barrier();
+}
 
 // Row r of a problem's R = group * q_len query rows: head and position.
 struct QueryRow {
@@ -224,13 +230,18 @@ __device__ __forceinline__ QueryRow query_row(int r, int q_len, int first_head) 
   return {first_head + g, r - g * q_len};
 }
 
-// This lane's row as MFMA B fragments (column lane % 32, chunks by lane half).
+// A row as MFMA B fragments (column lane % 32, chunks by lane half); a row that
+// is not valid may be read and counts as zeros.
 template <typename T, int DP, bool VEC>
 __device__ __forceinline__ void load_fragments(const typename Elem<T>::type* row, bool valid, int d, int half,
                                                u32x4 (&f)[Tile<T, DP>::NS]) {
 #pragma unroll
   for (int s = 0; s < Tile<T, DP>::NS; ++s) {
-    f[s] = valid ? load_chunk<T, VEC>(row, 2 * s + half, d) : zero_chunk();
+    if constexpr (VEC) {
+      f[s] = load_chunk_flat(row, (2 * s + half) * 16, d * static_cast<int>(sizeof(typename Elem<T>::type)), valid);
+    } else {
+      f[s] = load_chunk<T, VEC>(row, 2 * s + half, valid ? d : 0);
+    }
   }
 }
 
@@ -304,72 +315,41 @@ constexpr int tile_keys() {
   return Elem<T>::kChunk == 4 ? 32 : 64;
 }
 
-// ---------------------------------------------------------------------------
-// Forward: grid (problems, 128-row blocks, key splits), four waves of 32 rows.
+// Two waves per SIMD, so that one computes probabilities while the other's
+// products run; wide fp32 rows and element-wise loads need the registers of one.
 template <typename T, int DP, bool VEC>
-__global__ __launch_bounds__(256, (waves_per_simd<T, DP, VEC>())) void xattn_fwd_kernel(XAttnArgs a) {
-  using TL = Tile<T, DP>;
-  using E = typename Elem<T>::type;
-  constexpr int KT = tile_keys<T>();
-  constexpr int NB = KT / 32;
-  constexpr int TB = KT * TL::RB;
-  extern __shared__ __attribute__((aligned(16))) char smem[];  // K tiles at 0, TB; V tiles at 2 TB, 3 TB
-  const int tid = threadIdx.x;
-  const int lane = tid & 63;
-  const int half = lane >> 5;
-  const int b = blockIdx.x / a.kv_heads;
-  const int hk = blockIdx.x - b * a.kv_heads;
-  const int group = a.heads / a.kv_heads;
-  const int R = group * a.q_len;
-  const int r = blockIdx.y * 128 + (tid >> 6) * 32 + (lane & 31);
-  const bool valid = r < R;
-  const QueryRow qr = query_row(valid ? r : 0, a.q_len, hk * group);
-  const int len = keys_of(a, b);
-  int t0, t1;
-  tile_range((len + KT - 1) / KT, a.splits, blockIdx.z, &t0, &t1);
+constexpr int waves_per_simd() {
+  return DP == 128 && (Elem<T>::kChunk == 4 || !VEC) ? 1 : 2;
+}
 
-  Stream<T, DP, KT, VEC> ks, vs;
-  ks.init(static_cast<const E*>(a.k.p) + b * a.k.sb + hk * a.k.sh, a.k.ss, len, a.d, tid);
-  vs.init(static_cast<const E*>(a.v.p) + b * a.v.sb + hk * a.v.sh, a.v.ss, len, a.d, tid);
-  if (VEC && t0 < t1) {
-    ks.load(t0);
-    vs.load(t0);
-  }
+// The softmax state of a wave's 32 query rows (one a lane, in both lane halves)
+// over tiles of KT keys.  Scores and m in exp2 units.  m follows the running
+// maximum lazily: O and l are rescaled only when a tile's maximum passes it by
+// more than 8 (probabilities up to 256).
+template <typename T, int DP, int KT>
+struct FwdState {
+  using TL = Tile<T, DP>;
+  static constexpr int NB = KT / 32;
   u32x4 qf[TL::NS];
-  load_fragments<T, DP, VEC>(
-      static_cast<const E*>(a.q.p) + b * a.q.sb + qr.head * a.q.sh + static_cast<int64_t>(qr.pos) * a.q.ss, valid, a.d,
-      half, qf);
-  if (a.negate) {
-#pragma unroll
-    for (int s = 0; s < TL::NS; ++s) {
-      qf[s] = negated<T>(qf[s]);
-    }
-  }
   floatx16 o[TL::DT];
+  float m;
+  float l;
+  float c;
+  int len;
+  int lane;
+
+  __device__ __forceinline__ void init(float c_, int len_, int lane_) {
+    c = c_;
+    len = len_;
+    lane = lane_;
+    m = -INFINITY;
+    l = 0.0f;
 #pragma unroll
-  for (int t = 0; t < TL::DT; ++t) {
-    o[t] = zero16();
+    for (int t = 0; t < TL::DT; ++t) {
+      o[t] = zero16();
+    }
   }
-  // Scores and m in exp2 units.  m follows the running maximum lazily: O and l
-  // are rescaled only when a tile's maximum passes it by more than 8 (p <= 256).
-  float m = -INFINITY;
-  float l = 0.0f;
-  const float c = a.c;
-  for (int t = t0; t < t1; ++t) {
-    char* kl = smem + ((t - t0) & 1) * TB;
-    char* vl = kl + 2 * TB;
-    if (!VEC) {
-      ks.load(t);
-      vs.load(t);
-    }
-    ks.store(kl);
-    vs.store(vl);
-    __syncthreads();
-    if (VEC && t + 1 < t1) {
-      ks.load(t + 1);
-      vs.load(t + 1);
-    }
-    floatx16 s[NB];
+  __device__ __forceinline__ void scores(const char* kl, floatx16 (&s)[NB]) const {
 #pragma unroll
     for (int n = 0; n < NB; ++n) {
       s[n] = zero16();
@@ -378,9 +358,11 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP, VEC>())) void xattn_fwd
         s[n] = mma_rows<T>(TL::rows(kl, n * 32, f, lane), qf[f], s[n]);
       }
     }
-    float top = -INFINITY;
+  }
+  // Hides the keys past the row's length and moves m; returns what to subtract.
+  __device__ __forceinline__ float reference(int t, floatx16 (&s)[NB]) {
     if ((t + 1) * KT > len) {
-      const int lim = len - t * KT - 4 * half;
+      const int lim = len - t * KT - 4 * (lane >> 5);
 #pragma unroll
       for (int n = 0; n < NB; ++n) {
 #pragma unroll
@@ -391,6 +373,7 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP, VEC>())) void xattn_fwd
         }
       }
     }
+    float top = -INFINITY;
 #pragma unroll
     for (int n = 0; n < NB; ++n) {
 #pragma unroll
@@ -412,55 +395,299 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP, VEC>())) void xattn_fwd
         }
       }
     }
-    const float ref = m == -INFINITY ? 0.0f : m;
+    return m == -INFINITY ? 0.0f : m;
+  }
+  // Probabilities of a tile, in place; l sums them unrounded.
+  __device__ __forceinline__ void probabilities(floatx16 (&s)[NB], float ref) {
 #pragma unroll
     for (int n = 0; n < NB; ++n) {
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         s[n][i] = fast_exp2(fmaf(s[n][i], c, -ref));
+        l += s[n][i];
       }
+    }
+  }
+  // O += P V.  P goes to 16 bits for the matrix cores (an error of half a step a
+  // key, averaged over the keys).
+  __device__ __forceinline__ void values(const char* vl, const floatx16 (&s)[NB]) {
+#pragma unroll
+    for (int n = 0; n < NB; ++n) {
       if constexpr (TL::EC == 8) {
-        // P goes to 16 bits for the matrix cores (an error of half a step per
-        // key, averaged over the keys); l sums the rounded values, so the
-        // weights of a row still add up to one.
         u32x4 pk[2];
         pack_block<T>(s[n], pk);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          l = add_pair<T>(pk[i >> 2][i & 3], l);
-        }
         TL::transposed(vl, n * 32, pk, lane, o);
       } else {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          l += s[n][i];
-        }
         TL::transposed(vl, n * 32, s[n], lane, o);
       }
     }
   }
-  l = add_xor32(l);
+  // The same two with the next tile's scores between the exponentials: a product
+  // runs for 32 cycles while the wave issues the exponentials behind it (the
+  // scheduling barriers keep that order).
+  __device__ __forceinline__ void probabilities_and_scores(floatx16 (&s)[NB], float ref, const char* kn,
+                                                           floatx16 (&next)[NB]) {
+    constexpr int NQ = NB * TL::NS;
+    constexpr int EPM = NB * 16 / NQ;
+    u32x4 kf[3];
+    kf[0] = TL::rows(kn, 0, 0, lane);
+    kf[1] = TL::rows(kn, 1 / TL::NS * 32, 1 % TL::NS, lane);
+#pragma unroll
+    for (int g = 0; g < NQ; ++g) {
+      if (g + 2 < NQ) {
+        kf[(g + 2) % 3] = TL::rows(kn, (g + 2) / TL::NS * 32, (g + 2) % TL::NS, lane);
+      }
+      const int n = g / TL::NS;
+      const int f = g % TL::NS;
+      next[n] = mma_rows<T>(kf[g % 3], qf[f], f == 0 ? zero16() : next[n]);
+#pragma unroll
+      for (int e = 0; e < EPM; ++e) {
+        const int idx = g * EPM + e;
+        const float p = fast_exp2(fmaf(s[idx >> 4][idx & 15], c, -ref));
+        s[idx >> 4][idx & 15] = p;
+        l += p;
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+};
+
+// A row's result from its unnormalised o, m and l.
+__device__ __forceinline__ bool any_keys(float l) { return l > 0.0f || l != l; }
+
+// Forward: grid (problems, 128-row blocks, key splits), four waves of 32 rows.
+// K runs two tiles ahead of the probabilities, V one.
+template <typename T, int DP, bool VEC>
+__global__ __launch_bounds__(256, (waves_per_simd<T, DP, VEC>())) void xattn_fwd_kernel(XAttnArgs a) {
+  using TL = Tile<T, DP>;
+  using E = typename Elem<T>::type;
+  constexpr int KT = tile_keys<T>();
+  constexpr int NB = KT / 32;
+  constexpr int TB = KT * TL::RB;
+  extern __shared__ __attribute__((aligned(16))) char smem[];  // K tiles at 0, TB; V tiles at 2 TB, 3 TB
+  const int tid = threadIdx.x;
+  const int lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int half = lane >> 5;
+  const int b = blockIdx.x / a.kv_heads;
+  const int hk = blockIdx.x - b * a.kv_heads;
+  const int group = a.heads / a.kv_heads;
+  const int R = group * a.q_len;
+  const int r = blockIdx.y * 128 + wave * 32 + (lane & 31);
+  const bool valid = r < R;
+  const QueryRow qr = query_row(valid ? r : 0, a.q_len, hk * group);
+  const int len = keys_of(a, b);
+  int t0, t1;
+  tile_range((len + KT - 1) / KT, a.splits, blockIdx.z, &t0, &t1);
+
+  Stream<T, DP, KT, VEC, 4> ks, vs;
+  ks.init(static_cast<const E*>(a.k.p) + b * a.k.sb + hk * a.k.sh, a.k.ss, len, a.d, wave, lane);
+  vs.init(static_cast<const E*>(a.v.p) + b * a.v.sb + hk * a.v.sh, a.v.ss, len, a.d, wave, lane);
+  if (t0 < t1) {
+    ks.stage(t0, smem);
+    vs.stage(t0, smem + 2 * TB);
+    if (t0 + 1 < t1) {
+      ks.stage(t0 + 1, smem + TB);
+    }
+  }
+  FwdState<T, DP, KT> w;
+  w.init(a.c, len, lane);
+  load_fragments<T, DP, VEC>(
+      static_cast<const E*>(a.q.p) + b * a.q.sb + qr.head * a.q.sh + static_cast<int64_t>(qr.pos) * a.q.ss, valid, a.d,
+      half, w.qf);
+  if (a.negate) {
+#pragma unroll
+    for (int s = 0; s < TL::NS; ++s) {
+      w.qf[s] = negated<T>(w.qf[s]);
+    }
+  }
+  floatx16 sa[NB], sb[NB];
+  if (t0 < t1) {
+    arrive();
+    w.scores(smem, sa);
+    arrive();  // K buffer 0 is filled again next
+  }
+  auto step = [&](int t, floatx16 (&cur)[NB], floatx16 (&next)[NB]) {
+    const int at = (t - t0) & 1;
+    if (t + 2 < t1) {
+      ks.stage(t + 2, smem + at * TB);
+    }
+    if (t + 1 < t1) {
+      vs.stage(t + 1, smem + (3 - at) * TB);
+    }
+    const float ref = w.reference(t, cur);
+    // Past the last tile the scores are of a stale tile and go unused.
+    w.probabilities_and_scores(cur, ref, smem + (1 - at) * TB, next);
+    w.values(smem + (2 + at) * TB, cur);
+    arrive();
+  };
+  for (int t = t0; t < t1; t += 2) {
+    step(t, sa, sb);
+    if (t + 1 < t1) {
+      step(t + 1, sb, sa);
+    }
+  }
+  const float l = add_xor32(w.l);
   if (!valid) {
     return;
   }
   const size_t row = static_cast<size_t>(blockIdx.x) * R + r;
   if (a.splits > 1) {
     const size_t prow = static_cast<size_t>(blockIdx.z) * gridDim.x * R + row;
-    store_partial<TL::DT>(a.part + prow * DP, half, o, 1.0f);
+    store_partial<TL::DT>(a.part + prow * DP, half, w.o, 1.0f);
     if (half == 0) {
       float* ml = a.stats + prow * 2;
-      ml[0] = m;
+      ml[0] = w.m;
       ml[1] = l;
     }
     return;
   }
-  const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+  const float inv = any_keys(l) ? 1.0f / l : 0.0f;
   store_column<T, TL::DT, VEC>(static_cast<E*>(a.o.p) + b * a.o.sb + qr.head * a.o.sh +
                                    static_cast<int64_t>(qr.pos) * a.o.ss,
-                               a.d, half, o, inv);
+                               a.d, half, w.o, inv);
   if (a.lse != nullptr && half == 0) {
     a.lse[(static_cast<size_t>(b) * a.heads + qr.head) * a.q_len + qr.pos] =
-        l > 0.0f || l != l ? m * kLn2 + logf(l) : -INFINITY;
+        any_keys(l) ? w.m * kLn2 + logf(l) : -INFINITY;
+  }
+}
+
+// Forward of few rows: grid (problems, 32-row blocks, key splits).  The four
+// waves have the same 32 rows and take the split's tiles in turn, each with
+// tiles of its own in LDS and no barrier until their states are joined; K's
+// buffer is filled again as soon as the scores have read it, V's after O.
+template <typename T, int DP, bool VEC>
+__global__ __launch_bounds__(256, 1) void xattn_few_kernel(XAttnArgs a) {
+  using TL = Tile<T, DP>;
+  using E = typename Elem<T>::type;
+  constexpr int KT = tile_keys<T>();
+  constexpr int NB = KT / 32;
+  constexpr int TB = KT * TL::RB;
+  constexpr int SW = DP + 4;  // floats of a row of O in LDS
+  using St = Stream<T, DP, KT, VEC, 1>;
+  static_assert(4 * 32 * (SW + 2) * sizeof(float) <= 8u * TB, "the states fit where the tiles were");
+  extern __shared__ __attribute__((aligned(16))) char smem[];  // four waves' K and V tiles, then their states
+  const int tid = threadIdx.x;
+  const int lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int half = lane >> 5;
+  const int b = blockIdx.x / a.kv_heads;
+  const int hk = blockIdx.x - b * a.kv_heads;
+  const int group = a.heads / a.kv_heads;
+  const int R = group * a.q_len;
+  const int r = blockIdx.y * 32 + (lane & 31);
+  const bool valid = r < R;
+  const QueryRow qr = query_row(valid ? r : 0, a.q_len, hk * group);
+  const int len = keys_of(a, b);
+  int t0, t1;
+  tile_range((len + KT - 1) / KT, a.splits, blockIdx.z, &t0, &t1);
+  char* const kl = smem + wave * 2 * TB;
+  char* const vl = kl + TB;
+
+  St ks, vs;
+  ks.init(static_cast<const E*>(a.k.p) + b * a.k.sb + hk * a.k.sh, a.k.ss, len, a.d, 0, lane);
+  vs.init(static_cast<const E*>(a.v.p) + b * a.v.sb + hk * a.v.sh, a.v.ss, len, a.d, 0, lane);
+  FwdState<T, DP, KT> w;
+  w.init(a.c, len, lane);
+  load_fragments<T, DP, VEC>(
+      static_cast<const E*>(a.q.p) + b * a.q.sb + qr.head * a.q.sh + static_cast<int64_t>(qr.pos) * a.q.ss, valid, a.d,
+      half, w.qf);
+  if (a.negate) {
+#pragma unroll
+    for (int s = 0; s < TL::NS; ++s) {
+      w.qf[s] = negated<T>(w.qf[s]);
+    }
+  }
+  int t = t0 + wave;
+  if (t < t1) {
+    ks.stage(t, kl);
+    vs.stage(t, vl);
+  }
+  for (; t < t1; t += 4) {
+    // V's copies are the younger ones.
+    wait_vmcnt<VEC ? St::NI : 0>();
+    asm volatile("" ::: "memory");
+    floatx16 s[NB];
+    w.scores(kl, s);
+    wait_lgkmcnt<0>();
+    const bool more = t + 4 < t1;
+    if (more) {
+      ks.stage(t + 4, kl);
+    }
+    const float ref = w.reference(t, s);
+    w.probabilities(s, ref);
+    if (more) {
+      wait_vmcnt<VEC ? St::NI : 0>();
+    } else {
+      wait_vmcnt<0>();
+    }
+    asm volatile("" ::: "memory");
+    w.values(vl, s);
+    wait_lgkmcnt<0>();
+    if (more) {
+      vs.stage(t + 4, vl);
+    }
+  }
+  const float lw = add_xor32(w.l);
+  __syncthreads();
+  float* const so = reinterpret_cast<float*>(smem);
+  float* const sm = so + 4 * 32 * SW;  // [wave][m or l][row]
+  store_partial<TL::DT>(so + (wave * 32 + (lane & 31)) * SW, half, w.o, 1.0f);
+  if (half == 0) {
+    sm[wave * 64 + lane] = w.m;
+    sm[wave * 64 + 32 + lane] = lw;
+  }
+  __syncthreads();
+  // Eight threads a row join the waves' states.
+  const int row = tid >> 3;
+  const int d0 = (tid & 7) * 4;
+  const int r1 = blockIdx.y * 32 + row;
+  if (r1 >= R) {
+    return;
+  }
+  float m = -INFINITY;
+#pragma unroll
+  for (int x = 0; x < 4; ++x) {
+    m = fmaxf(m, sm[x * 64 + row]);
+  }
+  float l = 0.0f;
+  float f[4];
+#pragma unroll
+  for (int x = 0; x < 4; ++x) {
+    const float mx = sm[x * 64 + row];
+    f[x] = mx == -INFINITY ? 0.0f : fast_exp2(mx - m);
+    l = fmaf(f[x], sm[x * 64 + 32 + row], l);
+  }
+  const QueryRow q1 = query_row(r1, a.q_len, hk * group);
+  const size_t prow = (static_cast<size_t>(blockIdx.z) * gridDim.x + blockIdx.x) * R + r1;
+  const float inv = a.splits > 1 ? 1.0f : any_keys(l) ? 1.0f / l : 0.0f;
+  E* const out = static_cast<E*>(a.o.p) + b * a.o.sb + q1.head * a.o.sh + static_cast<int64_t>(q1.pos) * a.o.ss;
+#pragma unroll
+  for (int j = 0; j < TL::DT; ++j) {
+    float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const float4 p = *reinterpret_cast<const float4*>(so + (x * 32 + row) * SW + j * 32 + d0);
+      v[0] = fmaf(f[x], p.x, v[0]);
+      v[1] = fmaf(f[x], p.y, v[1]);
+      v[2] = fmaf(f[x], p.z, v[2]);
+      v[3] = fmaf(f[x], p.w, v[3]);
+    }
+    if (a.splits > 1) {
+      *reinterpret_cast<float4*>(a.part + prow * DP + j * 32 + d0) = make_float4(v[0], v[1], v[2], v[3]);
+    } else {
+      store4<T, VEC>(out, j * 32 + d0, a.d, v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
+    }
+  }
+  if ((tid & 7) != 0) {
+    return;
+  }
+  if (a.splits > 1) {
+    a.stats[prow * 2] = m;
+    a.stats[prow * 2 + 1] = l;
+  } else if (a.lse != nullptr) {
+    a.lse[(static_cast<size_t>(b) * a.heads + q1.head) * a.q_len + q1.pos] =
+        any_keys(l) ? m * kLn2 + logf(l) : -INFINITY;
   }
 }
 
@@ -482,11 +709,13 @@ __global__ __launch_bounds__(256) void xattn_join_kernel(XAttnArgs a) {
   const QueryRow qr = query_row(static_cast<int>(row - static_cast<size_t>(problem) * R), a.q_len,
                                 (problem - b * a.kv_heads) * group);
   float m = -INFINITY;
+#pragma unroll 4
   for (int z = 0; z < a.splits; ++z) {
     m = fmaxf(m, a.stats[(z * rows + row) * 2]);
   }
   float l = 0.0f;
   float o[PL] = {};
+#pragma unroll 4
   for (int z = 0; z < a.splits; ++z) {
     const float* ml = a.stats + (z * rows + row) * 2;
     const float w = ml[0] == -INFINITY ? 0.0f : fast_exp2(ml[0] - m);
@@ -496,7 +725,7 @@ __global__ __launch_bounds__(256) void xattn_join_kernel(XAttnArgs a) {
       o[i] = fmaf(w, a.part[(z * rows + row) * DP + i * 64 + lane], o[i]);
     }
   }
-  const bool any = l > 0.0f || l != l;
+  const bool any = any_keys(l);
   const float inv = any ? 1.0f / l : 0.0f;
   E* out = static_cast<E*>(a.o.p) + b * a.o.sb + qr.head * a.o.sh + static_cast<int64_t>(qr.pos) * a.o.ss;
 #pragma unroll
@@ -535,24 +764,25 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP, VEC>())) void xattn_dq_
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int tid = threadIdx.x;
   const int lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int half = lane >> 5;
   const int b = blockIdx.x / a.kv_heads;
   const int hk = blockIdx.x - b * a.kv_heads;
   const int group = a.heads / a.kv_heads;
   const int R = group * a.q_len;
-  const int r = blockIdx.y * 128 + (tid >> 6) * 32 + (lane & 31);
+  const int r = blockIdx.y * 128 + wave * 32 + (lane & 31);
   const bool valid = r < R;
   const QueryRow qr = query_row(valid ? r : 0, a.q_len, hk * group);
   const int len = keys_of(a, b);
   int t0, t1;
   tile_range((len + KT - 1) / KT, a.splits, blockIdx.z, &t0, &t1);
 
-  Stream<T, DP, KT, VEC> ks, vs;
-  ks.init(static_cast<const E*>(a.k.p) + b * a.k.sb + hk * a.k.sh, a.k.ss, len, a.d, tid);
-  vs.init(static_cast<const E*>(a.v.p) + b * a.v.sb + hk * a.v.sh, a.v.ss, len, a.d, tid);
-  if (VEC && t0 < t1) {
-    ks.load(t0);
-    vs.load(t0);
+  Stream<T, DP, KT, VEC, 4> ks, vs;
+  ks.init(static_cast<const E*>(a.k.p) + b * a.k.sb + hk * a.k.sh, a.k.ss, len, a.d, wave, lane);
+  vs.init(static_cast<const E*>(a.v.p) + b * a.v.sb + hk * a.v.sh, a.v.ss, len, a.d, wave, lane);
+  if (t0 < t1) {
+    ks.stage(t0, smem);
+    vs.stage(t0, smem + 2 * TB);
   }
   const int64_t pos = qr.pos;
   u32x4 qf[TL::NS], gf[TL::NS];
@@ -600,23 +830,20 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP, VEC>())) void xattn_dq_
     dq[t] = zero16();
   }
   const float c = a.c;
+  if (t0 < t1) {
+    arrive();
+  }
   for (int t = t0; t < t1; ++t) {
-    char* kl = smem + ((t - t0) & 1) * TB;
-    char* vl = kl + 2 * TB;
-    if (!VEC) {
-      ks.load(t);
-      vs.load(t);
-    }
-    ks.store(kl);
-    vs.store(vl);
-    __syncthreads();
-    if (VEC && t + 1 < t1) {
-      ks.load(t + 1);
-      vs.load(t + 1);
+    const int at = (t - t0) & 1;
+    const char* kl = smem + at * TB;
+    const char* vl = kl + 2 * TB;
+    if (t + 1 < t1) {
+      ks.stage(t + 1, smem + (1 - at) * TB);
+      vs.stage(t + 1, smem + (3 - at) * TB);
     }
     const int lim = len - t * KT - 4 * half;
     const bool tail = (t + 1) * KT > len;
-#pragma unroll
+#pragma unroll 1
     for (int n = 0; n < NB; ++n) {
       floatx16 s = zero16();
       floatx16 dp = zero16();
@@ -646,6 +873,7 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP, VEC>())) void xattn_dq_
         TL::transposed(kl, n * 32, s, lane, dq);
       }
     }
+    arrive();
   }
   if (!valid) {
     return;
@@ -665,60 +893,82 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP, VEC>())) void xattn_dq_
                                dq, f);
 }
 
+constexpr int kQueryTile = 32;
+template <typename T, int DP>
+constexpr size_t dkv_lds_bytes() {
+  return (4 * kQueryTile + 128) * Tile<T, DP>::RB + 6 * kQueryTile * sizeof(float);
+}
+
 // dK and dV: grid (problems, 128-key blocks, splits of the query tiles), four
-// waves of 32 keys; Q and dO stream.
+// waves of 32 keys; Q and dO stream.  The workgroup's own rows of V stay in LDS:
+// in registers beside K's and two accumulators they would leave room for one
+// wave on a SIMD, whose products then wait for its exponentials (16-bit, 64
+// heads of 2048 x 1500 x 128: 465 us).
 template <typename T, int DP, bool VEC>
-__global__ __launch_bounds__(256, 1) void xattn_dkv_kernel(XAttnArgs a) {
+__global__ __launch_bounds__(256, (VEC && Elem<T>::kChunk == 8 ? 2 : 1)) void xattn_dkv_kernel(XAttnArgs a) {
   using TL = Tile<T, DP>;
   using E = typename Elem<T>::type;
-  constexpr int KT = tile_keys<T>();
-  constexpr int NB = KT / 32;
+  constexpr int KT = kQueryTile;
   constexpr int TB = KT * TL::RB;
-  extern __shared__ __attribute__((aligned(16))) char smem[];  // Q, dO tiles, then lse, delta and exponents
+  extern __shared__ __attribute__((aligned(16))) char smem[];  // Q, dO tiles, lse, delta and exponents, V
   float* const st = reinterpret_cast<float*>(smem + 4 * TB);   // [2][3][KT]
+  char* const own = smem + 4 * TB + 6 * KT * sizeof(float);
   const int tid = threadIdx.x;
   const int lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int half = lane >> 5;
   const int b = blockIdx.x / a.kv_heads;
   const int hk = blockIdx.x - b * a.kv_heads;
   const int group = a.heads / a.kv_heads;
-  const int key = blockIdx.y * 128 + (tid >> 6) * 32 + (lane & 31);
+  const int key = blockIdx.y * 128 + wave * 32 + (lane & 31);
   const int len = keys_of(a, b);
   const bool valid = key < len;
   // Tiles: those of the group's heads, one after the other.
   const int per_head = (a.q_len + KT - 1) / KT;
   int t0, t1;
-  tile_range(blockIdx.y * 128 < len ? group * per_head : 0, a.splits, blockIdx.z, &t0, &t1);
+  tile_range(static_cast<int>(blockIdx.y) * 128 < len ? group * per_head : 0, a.splits, blockIdx.z, &t0, &t1);
 
-  Stream<T, DP, KT, VEC> qs, gs;
+  Stream<T, DP, KT, VEC, 4> qs, gs;
   float rl = 0.0f, rd = 0.0f, re = 0.0f;
-  auto load = [&](int t) {
+  // Starts moving tile t; its rows' statistics stay in registers until `keep`.
+  auto stage = [&](int t, int buf) {
     const int g = t / per_head;
     const int tile = t - g * per_head;
     const int head = hk * group + g;
-    qs.init(static_cast<const E*>(a.q.p) + b * a.q.sb + head * a.q.sh, a.q.ss, a.q_len, a.d, tid);
-    gs.init(static_cast<const E*>(a.go.p) + b * a.go.sb + head * a.go.sh, a.go.ss, a.q_len, a.d, tid);
-    qs.load(tile);
-    gs.load(tile);
     if (tid < KT) {
       const int pos = tile * KT + tid;
       const bool in = pos < a.q_len;
       const size_t row = (static_cast<size_t>(b) * a.heads + head) * a.q_len + (in ? pos : 0);
+      const float* dr = a.delta + 2 * row;
       // A row past the end has probabilities of zero.
       rl = in ? a.lse[row] * kLog2e : INFINITY;
-      rd = in ? a.delta[2 * row] : 0.0f;
-      re = in ? a.delta[2 * row + 1] : kNoExponent;
+      rd = in ? dr[0] : 0.0f;
+      re = in ? dr[1] : kNoExponent;
+    }
+    qs.init(static_cast<const E*>(a.q.p) + b * a.q.sb + head * a.q.sh, a.q.ss, a.q_len, a.d, wave, lane);
+    gs.init(static_cast<const E*>(a.go.p) + b * a.go.sb + head * a.go.sh, a.go.ss, a.q_len, a.d, wave, lane);
+    qs.stage(tile, smem + buf * TB);
+    gs.stage(tile, smem + (2 + buf) * TB);
+  };
+  auto keep = [&](int buf) {
+    if (tid < KT) {
+      float* sl = st + buf * 3 * KT;
+      sl[tid] = rl;
+      sl[KT + tid] = rd;
+      sl[2 * KT + tid] = re;
     }
   };
-  if (VEC && t0 < t1) {
-    load(t0);
-  }
-  u32x4 kf[TL::NS], vf[TL::NS];
+  u32x4 kf[TL::NS];
   const int64_t krow = valid ? key : 0;
+  const E* const vbase = static_cast<const E*>(a.v.p) + b * a.v.sb + hk * a.v.sh;
+  if (t0 < t1) {
+    stage(t0, 0);
+    Stream<T, DP, 128, VEC, 4> vs;
+    vs.init(vbase, a.v.ss, len, a.d, wave, lane);
+    vs.stage(blockIdx.y, own);
+  }
   load_fragments<T, DP, VEC>(static_cast<const E*>(a.k.p) + b * a.k.sb + hk * a.k.sh + krow * a.k.ss, valid, a.d, half,
                              kf);
-  load_fragments<T, DP, VEC>(static_cast<const E*>(a.v.p) + b * a.v.sb + hk * a.v.sh + krow * a.v.ss, valid, a.d, half,
-                             vf);
   if (a.negate) {
 #pragma unroll
     for (int s = 0; s < TL::NS; ++s) {
@@ -733,30 +983,23 @@ __global__ __launch_bounds__(256, 1) void xattn_dkv_kernel(XAttnArgs a) {
   }
   int ex = kNoExponent;  // fp16: dk is held at 2^-ex
   const float c = a.c;
+  if (t0 < t1) {
+    keep(0);
+    arrive();
+  }
   for (int t = t0; t < t1; ++t) {
     const int buf = (t - t0) & 1;
-    char* ql = smem + buf * TB;
-    char* gl = ql + 2 * TB;
-    float* sl = st + buf * 3 * KT;
-    if (!VEC) {
-      load(t);
-    }
-    qs.store(ql);
-    gs.store(gl);
-    if (tid < KT) {
-      sl[tid] = rl;
-      sl[KT + tid] = rd;
-      sl[2 * KT + tid] = re;
-    }
-    __syncthreads();
-    if (VEC && t + 1 < t1) {
-      load(t + 1);
+    const char* ql = smem + buf * TB;
+    const char* gl = ql + 2 * TB;
+    const float* sl = st + buf * 3 * KT;
+    if (t + 1 < t1) {
+      stage(t + 1, 1 - buf);
     }
     float down = 1.0f;
     if constexpr (__is_same(T, F16)) {
-      float e = lane < KT ? sl[2 * KT + lane] : kNoExponent;
+      float e = sl[2 * KT + (lane & (KT - 1))];
 #pragma unroll
-      for (int x = 32; x > 0; x >>= 1) {
+      for (int x = KT / 2; x > 0; x >>= 1) {
         e = fmaxf(e, __shfl_xor(e, x));
       }
       const int et = __builtin_amdgcn_readfirstlane(static_cast<int>(e));
@@ -773,40 +1016,41 @@ __global__ __launch_bounds__(256, 1) void xattn_dkv_kernel(XAttnArgs a) {
       }
       down = power_of_two(-ex);
     }
+    floatx16 s = zero16();
+    floatx16 dp = zero16();
 #pragma unroll
-    for (int n = 0; n < NB; ++n) {
-      floatx16 s = zero16();
-      floatx16 dp = zero16();
+    for (int f = 0; f < TL::NS; ++f) {
+      s = mma_rows<T>(TL::rows(ql, 0, f, lane), kf[f], s);
+      dp = mma_rows<T>(TL::rows(gl, 0, f, lane), TL::rows(own, wave * 32, f, lane), dp);
+    }
 #pragma unroll
-      for (int f = 0; f < TL::NS; ++f) {
-        s = mma_rows<T>(TL::rows(ql, n * 32, f, lane), kf[f], s);
-        dp = mma_rows<T>(TL::rows(gl, n * 32, f, lane), vf[f], dp);
-      }
+    for (int g = 0; g < 4; ++g) {
+      const int r0 = 8 * g + 4 * half;
+      const float4 l4 = *reinterpret_cast<const float4*>(sl + r0);
+      const float4 d4 = *reinterpret_cast<const float4*>(sl + KT + r0);
+      const float lv[4] = {l4.x, l4.y, l4.z, l4.w};
+      const float dl[4] = {d4.x, d4.y, d4.z, d4.w};
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const int r0 = n * 32 + 8 * g + 4 * half;
-        const float4 l4 = *reinterpret_cast<const float4*>(sl + r0);
-        const float4 d4 = *reinterpret_cast<const float4*>(sl + KT + r0);
-        const float lv[4] = {l4.x, l4.y, l4.z, l4.w};
-        const float dl[4] = {d4.x, d4.y, d4.z, d4.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float p = fast_exp2(fmaf(s[4 * g + i], c, -lv[i]));
-          s[4 * g + i] = p;
-          dp[4 * g + i] = p * (dp[4 * g + i] - dl[i]) * down;
-        }
-      }
-      if constexpr (TL::EC == 8) {
-        u32x4 pk[2];
-        pack_block<T>(s, pk);
-        TL::transposed(gl, n * 32, pk, lane, dv);
-        pack_block<T>(dp, pk);
-        TL::transposed(ql, n * 32, pk, lane, dk);
-      } else {
-        TL::transposed(gl, n * 32, s, lane, dv);
-        TL::transposed(ql, n * 32, dp, lane, dk);
+      for (int i = 0; i < 4; ++i) {
+        const float p = fast_exp2(fmaf(s[4 * g + i], c, -lv[i]));
+        s[4 * g + i] = p;
+        dp[4 * g + i] = p * (dp[4 * g + i] - dl[i]) * down;
       }
     }
+    if constexpr (TL::EC == 8) {
+      u32x4 pk[2];
+      pack_block<T>(s, pk);
+      TL::transposed(gl, 0, pk, lane, dv);
+      pack_block<T>(dp, pk);
+      TL::transposed(ql, 0, pk, lane, dk);
+    } else {
+      TL::transposed(gl, 0, s, lane, dv);
+      TL::transposed(ql, 0, dp, lane, dk);
+    }
+    if (t + 1 < t1) {
+      keep(1 - buf);
+    }
+    arrive();
   }
   if (key >= a.kv_len) {
     return;
@@ -854,6 +1098,7 @@ __global__ __launch_bounds__(256) void xattn_sum_kernel(const float* __restrict_
   const int b = problem / heads;
   const XTensor x = blockIdx.y == 0 ? first : second;
   float s[PL] = {};
+#pragma unroll 8
   for (int z = 0; z < splits; ++z) {
     const float* p = part + ((static_cast<size_t>(z) * planes + blockIdx.y) * rows + row) * DP + lane;
 #pragma unroll
@@ -896,6 +1141,11 @@ hipError_t launch(XAttnStep step, const XAttnArgs& a, hipStream_t stream) {
   const unsigned z = static_cast<unsigned>(a.splits);
   constexpr size_t lds = tiles_bytes<T, DP>();
   const dim3 by_rows(problems, static_cast<unsigned>((rows + 127) / 128), z);
+  if (step == XAttnStep::kForward && a.few) {
+    static const hipError_t allowed = LC_XATTN_ALLOW((xattn_few_kernel<T, DP, VEC>), 2 * lds);
+    return launch_lds(xattn_few_kernel<T, DP, VEC>, allowed,
+                      dim3(problems, static_cast<unsigned>((rows + 31) / 32), z), 2 * lds, a, stream);
+  }
   if (step == XAttnStep::kForward) {
     static const hipError_t allowed = LC_XATTN_ALLOW((xattn_fwd_kernel<T, DP, VEC>), lds);
     return launch_lds(xattn_fwd_kernel<T, DP, VEC>, allowed, by_rows, lds, a, stream);
@@ -904,10 +1154,10 @@ hipError_t launch(XAttnStep step, const XAttnArgs& a, hipStream_t stream) {
     static const hipError_t allowed = LC_XATTN_ALLOW((xattn_dq_kernel<T, DP, VEC>), lds);
     return launch_lds(xattn_dq_kernel<T, DP, VEC>, allowed, by_rows, lds, a, stream);
   }
-  constexpr size_t more = lds + 6 * tile_keys<T>() * sizeof(float);
-  static const hipError_t allowed = LC_XATTN_ALLOW((xattn_dkv_kernel<T, DP, VEC>), more);
-  return launch_lds(xattn_dkv_kernel<T, DP, VEC>, allowed, dim3(problems, static_cast<unsigned>((a.kv_len + 127) / 128), z),
-                    more, a, stream);
+  constexpr size_t kv_lds = dkv_lds_bytes<T, DP>();
+  static const hipError_t allowed = LC_XATTN_ALLOW((xattn_dkv_kernel<T, DP, VEC>), kv_lds);
+  return launch_lds(xattn_dkv_kernel<T, DP, VEC>, allowed,
+                    dim3(problems, static_cast<unsigned>((a.kv_len + 127) / 128), z), kv_lds, a, stream);
 }
 #undef LC_XATTN_ALLOW
 

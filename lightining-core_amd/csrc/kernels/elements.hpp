@@ -89,6 +89,46 @@ __device__ __forceinline__ u32x4 load_chunk(const typename Elem<T>::type* row, i
   return r;
 }
 
+// The same of an aligned row without a branch around the load, for many chunks
+// that are needed at once: past the end it reads the row's first chunk and
+// drops it, as it does the whole row when `on` is false.
+__device__ __forceinline__ u32x4 load_chunk_flat(const void* row, int at_bytes, int row_bytes, bool on) {
+  const bool in = at_bytes < row_bytes;
+  const u32x4 v = *reinterpret_cast<const u32x4*>(static_cast<const char*>(row) + (in ? at_bytes : 0));
+  u32x4 r;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    r[i] = in && on ? v[i] : 0u;
+  }
+  return r;
+}
+
+// A buffer descriptor of `bytes` bytes from p (wave-uniform): loads at offsets
+// past its end return zero.
+__device__ __forceinline__ u32x4 buffer_of(const void* p, int bytes) {
+  const uint64_t a = reinterpret_cast<uint64_t>(p);
+  u32x4 r;
+  r[0] = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(a));
+  r[1] = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(a >> 32)) & 0xffffu;
+  r[2] = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(bytes));
+  r[3] = 0x00027000u;
+  return r;
+}
+
+// 16 bytes of each lane from offset voff of the buffer to LDS at lds + 16 lane;
+// zeros where the offset is past the buffer's end.  In asm for the reason given
+// at load_lds16_sbase (kcommon.hpp): the compiler's own copies make every later
+// LDS wait a full one.  The caller waits with wait_vmcnt.  The s_nop is the five
+// wait states that a VMEM read of an SGPR needs after a VALU wrote it (the
+// descriptor may come from v_readfirstlane), and the one that an LDS copy needs
+// after a write of M0.
+__device__ __forceinline__ void load_lds16_buffer(uint32_t voff, u32x4 buffer, uint32_t lds) {
+  asm volatile("s_nop 4\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds"
+               :
+               : "v"(voff), "s"(buffer), "{m0}"(lds)
+               : "memory");
+}
+
 // v summed over lanes l and l ^ 32.
 __device__ __forceinline__ float add_xor32(float v) {
   const uint32_t u = __builtin_bit_cast(uint32_t, v);

@@ -89,7 +89,7 @@ Status store(const lcKvCache* cache, std::size_t batch, std::size_t kv_len, lcDa
   }
   LC_TRY(checkTable(c, table, batch, need, stride));
   DeviceCall call;
-  LC_TRY(call.open(kOp));
+  LC_TRY(call.open(kOp, c.trusted_pointers != 0));
   if (batch == 0 || kv_len == 0) {
     return Status::kSuccess;
   }
@@ -165,7 +165,7 @@ Status attention(const lcKvCache* cache, const lcKvAttentionConfig* cfg, const l
                     &o_aligned));
   LC_TRY(checkTable(c, table, cfg->batch, cfg->table_width, stride));
   DeviceCall call;
-  LC_TRY(call.open(kOp));
+  LC_TRY(call.open(kOp, c.trusted_pointers != 0));
   if (plan.rows == 0) {
     return Status::kSuccess;
   }

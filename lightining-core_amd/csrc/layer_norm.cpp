@@ -95,7 +95,7 @@ Status forward(const lcLayerNormConfig* cfg, const void* x, std::int64_t x_strid
     return fail(Status::kInvalidValue, "layer norm: mean and rstd are stored together or not at all");
   }
   DeviceCall call;
-  LC_TRY(call.open(kOp));
+  LC_TRY(call.open(kOp, c.trusted_pointers != 0));
   if (c.rows == 0) {
     return Status::kSuccess;
   }
@@ -135,7 +135,7 @@ Status backward(const lcLayerNormConfig* cfg, const void* dy, std::int64_t dy_st
     return fail(Status::kInvalidValue, "layer norm: the backward pass needs the forward's mean and rstd");
   }
   DeviceCall call;
-  LC_TRY(call.open(kOp));
+  LC_TRY(call.open(kOp, c.trusted_pointers != 0));
   const std::size_t need = partBytes(c);
   if (need != 0 && (workspace == nullptr || workspace_bytes < need)) {
     return fail(Status::kInvalidValue, "layer norm: the workspace needs " + std::to_string(need) + " bytes, " +

@@ -38,87 +38,98 @@ def _is_torch(x) -> bool:
 
 
 class _Torch:
-    """A call on torch tensors of one device."""
+    """Calls on torch tensors of one device.  One object per device: it keeps
+    nothing of a call."""
 
-    _dtypes = None
-    _names = {N.LC_DTYPE_F32: "float32", N.LC_DTYPE_BF16: "bfloat16", N.LC_DTYPE_F16: "float16"}
+    def __init__(self, torch, index):
+        own = ctypes.c_int()
+        _check(_lib().lcHipDeviceIndex(_byref(own)))
+        if index != own.value:
+            raise ValueError(f"the tensors are on cuda:{index}, the library computes on cuda:{own.value}")
+        self.torch, self.index = torch, index
+        self.device = torch.device("cuda", index)
+        self._dtypes = {torch.float32: N.LC_DTYPE_F32, torch.bfloat16: N.LC_DTYPE_BF16,
+                        torch.float16: N.LC_DTYPE_F16}
+        self._types = {v: k for k, v in self._dtypes.items()}
+        self._tensor = torch.Tensor
+        self._empty = torch.empty
+        self._int32, self._float32 = torch.int32, torch.float32
+        # The stream's handle without a Stream object around it (2 us a call less).
+        raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+        self._raw = raw or (lambda i: torch.cuda.current_stream(i).cuda_stream)
 
-    def __init__(self, first):
-        torch = self.torch = sys.modules["torch"]
-        if _Torch._dtypes is None:
-            _Torch._dtypes = {torch.float32: N.LC_DTYPE_F32, torch.bfloat16: N.LC_DTYPE_BF16,
-                              torch.float16: N.LC_DTYPE_F16}
-        self.device = first.device
-        if self.device.type != "cuda":
-            raise ValueError("torch tensors must be in GPU memory (pass numpy arrays for host data)")
-        self.stream = torch.cuda.current_stream(self.device).cuda_stream
-        self._kept = []
+    @property
+    def stream(self):
+        return self._raw(self.index)
 
     def take(self, x, name):
-        """x itself, when it is a tensor of this call's device."""
-        if not _is_torch(x):
+        """x itself, when it is a tensor of this device."""
+        if not isinstance(x, self._tensor):
             raise ValueError(f"{name} must be a torch tensor, as the other arguments are")
-        if x.device != self.device:
+        if not x.is_cuda or x.get_device() != self.index:
             raise ValueError(f"{name} is on {x.device}, the other tensors on {self.device}")
         return x
 
     def dtype(self, x, name):
-        try:
-            return self._dtypes[x.dtype]
-        except KeyError:
-            raise ValueError(f"{name} must be float32, bfloat16 or float16") from None
+        got = self._dtypes.get(x.dtype)
+        if got is None:
+            raise ValueError(f"{name} must be float32, bfloat16 or float16")
+        return got
 
     def ints(self, x, name):
-        x = self.take(x, name)
-        if x.dtype != self.torch.int32:
+        self.take(x, name)
+        if x.dtype is not self._int32:
             raise ValueError(f"{name} must be int32")
         return x
 
-    def strides(self, x):
+    @staticmethod
+    def strides(x):
         return x.stride()
 
-    def addr(self, x):
+    @staticmethod
+    def addr(x):
         return x.data_ptr()
 
-    def empty(self, shape, dtype):
-        return self.torch.empty(shape, dtype=getattr(self.torch, self._names[dtype]), device=self.device)
+    def empty(self, like, shape, dtype):
+        return like.new_empty(shape, dtype=self._types[dtype])
 
     def empty_like(self, x):
         """x's type, shape and order of dimensions; the last one contiguous."""
         y = self.torch.empty_like(x)
-        if y.shape[-1] > 1 and y.stride(-1) != 1:
-            y = self.torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        return y.detach() if y.requires_grad else y
+        if y.stride(-1) != 1 and y.shape[-1] > 1:
+            y = self._empty(x.shape, dtype=x.dtype, device=self.device)
+        return y
+
+    def empty_contiguous(self, x):
+        return self.torch.empty_like(x) if x.is_contiguous() else x.new_empty(x.shape)
 
     def codes(self, x, name):
-        x = self.take(x, name)
-        if x.dtype != self.torch.uint8 and x.dtype != self.torch.float8_e4m3fn:
+        self.take(x, name)
+        if x.dtype is not self.torch.uint8 and x.dtype is not self.torch.float8_e4m3fn:
             raise ValueError(f"{name} must be uint8 or float8_e4m3fn")
         if not x.is_contiguous():
             raise ValueError(f"{name} must be contiguous")
         return x
 
     def scales(self, x, name):
-        x = self.take(x, name)
-        if x.dtype != self.torch.float32 or not x.is_contiguous():
+        self.take(x, name)
+        if x.dtype is not self._float32 or not x.is_contiguous():
             raise ValueError(f"{name} must be contiguous float32")
         return x
 
-    def is_contiguous(self, x):
+    @staticmethod
+    def is_contiguous(x):
         return x.is_contiguous()
 
     def workspace(self, nbytes):
-        """Scratch of this call: the allocator hands it out again only to work
-        queued behind this call's on the same stream."""
-        if nbytes == 0:
-            return None
-        w = self.torch.empty(nbytes, dtype=self.torch.uint8, device=self.device)
-        self._kept.append(w)
-        return w.data_ptr()
+        """Scratch of a call, held by the caller until the call is queued: the
+        allocator hands it out again only to work queued behind it on the same
+        stream."""
+        return self._empty(nbytes, dtype=self.torch.uint8, device=self.device) if nbytes else None
 
     def rows(self, x, name):
         """(row count, row stride) of x seen as rows of its last dimension."""
-        if x.dim() == 2:
+        if x.ndim == 2:
             return x.shape[0], x.stride(0)
         try:
             v = x.view(-1, x.shape[-1]) if x.numel() else x.reshape(0, x.shape[-1])
@@ -126,8 +137,22 @@ class _Torch:
             raise ValueError(f"{name}'s leading dimensions must collapse to rows of one stride") from None
         return v.shape[0], v.stride(0)
 
-    def finish(self, *results):
+    @staticmethod
+    def finish(*results):
         return results
+
+
+_torch_calls = {}
+
+
+def _torch_call(x):
+    if not x.is_cuda:
+        raise ValueError("torch tensors must be in GPU memory (pass numpy arrays for host data)")
+    index = x.get_device()
+    call = _torch_calls.get(index)
+    if call is None:
+        call = _torch_calls[index] = _Torch(sys.modules["torch"], index)
+    return call
 
 
 class _Numpy:
@@ -137,9 +162,8 @@ class _Numpy:
     _dtypes = {np.dtype(np.float32): N.LC_DTYPE_F32, np.dtype(np.float16): N.LC_DTYPE_F16}
     _types = {N.LC_DTYPE_F32: np.float32, N.LC_DTYPE_F16: np.float16}
 
-    def __init__(self, first):
+    def __init__(self):
         self._bufs = {}   # id(array) -> (device address, array)
-        self._kept = []
         s = ctypes.c_void_p()
         _check(_lib().lcHipBackendStream(_byref(s)))
         self.stream = s.value
@@ -150,9 +174,7 @@ class _Numpy:
     def close(self):
         for addr, _ in self._bufs.values():
             _lib().lcFree(addr)
-        for addr in self._kept:
-            _lib().lcFree(addr)
-        self._bufs, self._kept = {}, []
+        self._bufs = {}
 
     def take(self, x, name):
         if _is_torch(x):
@@ -191,11 +213,13 @@ class _Numpy:
             _check(_lib().lcMemcpy(p, x.ctypes.data, x.nbytes, N.LC_MEMCPY_HOST_TO_DEVICE))
         return got[0]
 
-    def empty(self, shape, dtype):
+    def empty(self, like, shape, dtype):
         return np.zeros(shape, self._types[dtype])
 
     def empty_like(self, x):
         return np.zeros(x.shape, x.dtype)
+
+    empty_contiguous = empty_like
 
     def codes(self, x, name):
         if not isinstance(x, np.ndarray) or x.dtype != np.uint8 or not x.flags.c_contiguous:
@@ -211,10 +235,7 @@ class _Numpy:
         return x.flags.c_contiguous
 
     def workspace(self, nbytes):
-        if nbytes == 0:
-            return None
-        self._kept.append(self._malloc(nbytes))
-        return self._kept[-1]
+        return np.empty(nbytes, np.uint8) if nbytes else None
 
     def rows(self, x, name):
         n = x.shape[-1]
@@ -230,19 +251,23 @@ class _Numpy:
 
 
 def _call_of(first):
-    return _Torch(first) if _is_torch(first) else _Numpy(first)
+    return _torch_call(first) if _is_torch(first) else _Numpy()
 
 
 def _tensor4(call, x, name):
     """The library's view of a [batch, heads, rows, d] tensor."""
-    sb, sh, ss, sd = call.strides(x)
-    if sd != 1 and x.shape[3] > 1:
+    st = call.strides(x)
+    if st[3] != 1 and x.shape[3] > 1:
         raise ValueError(f"{name}'s last dimension must be contiguous")
-    return N.DeviceTensor(call.addr(x), sb, sh, ss)
+    return _byref(N.DeviceTensor(call.addr(x), st[0], st[1], st[2]))
+
+
+def _addr(call, x):
+    return None if x is None else call.addr(x)
 
 
 def _same(x, shape, name):
-    if tuple(x.shape) != tuple(shape):
+    if x.shape != shape:
         raise ValueError(f"{name} has shape {tuple(x.shape)}, expected {tuple(shape)}")
 
 
@@ -287,31 +312,32 @@ def _out(call, out, like, name):
     return out
 
 
-@functools.lru_cache(maxsize=512)
-def _xattn_plan(*key):
-    """The configuration of a shape and its workspaces' sizes."""
-    cfg = N.CrossAttentionConfig(*key)
+@functools.lru_cache(maxsize=1024)
+def _xattn_plan(q_shape, k_shape, dtype, scale):
+    """The configuration of a pair of shapes and its workspaces' sizes."""
+    b, hq, sq, d = q_shape
+    bk, hkv, sk, dk = k_shape
+    if bk != b or dk != d:
+        raise ValueError("q and k must agree in batch and head_dim")
+    if hkv == 0 or hq % hkv:
+        raise ValueError("q's heads must be a multiple of k's")
+    cfg = N.CrossAttentionConfig(b, hq, hkv, sq, sk, d, dtype, scale, 1)
     got = []
     for backward in (0, 1):
         n = ctypes.c_size_t()
         _check(_lib().lcCrossAttentionWorkspaceSize(_byref(cfg), backward, _byref(n)))
         got.append(n.value)
-    return cfg, got[0], got[1]
+    return _byref(cfg), got[0], got[1]
 
 
 def _xattn_inputs(call, q, k, v, scale):
     q, k, v = call.take(q, "q"), call.take(k, "k"), call.take(v, "v")
-    b, hq, sq, d = _four(q, "q")
-    bk, hkv, sk, dk = _four(k, "k")
-    if bk != b or dk != d:
-        raise ValueError("q and k must agree in batch and head_dim")
-    if hkv == 0 or hq % hkv:
-        raise ValueError("q's heads must be a multiple of k's")
-    _same(v, k.shape, "v")
+    shape = _four(k, "k")
+    if v.shape != shape:
+        _same(v, shape, "v")
     if not (q.dtype == k.dtype == v.dtype):
         raise ValueError("q, k and v must have one type")
-    plan = _xattn_plan(b, hq, hkv, sq, sk, d, call.dtype(q, "q"), _scale(scale))
-    return q, k, v, plan
+    return q, k, v, _xattn_plan(_four(q, "q"), shape, call.dtype(q, "q"), _scale(scale))
 
 
 def cross_attention(q, k, v, kv_lengths=None, *, scale=None, return_lse=False, out=None):
@@ -329,11 +355,11 @@ def cross_attention(q, k, v, kv_lengths=None, *, scale=None, return_lse=False, o
     q, k, v, (cfg, nbytes, _) = _xattn_inputs(call, q, k, v, scale)
     lengths = _lengths(call, kv_lengths, q.shape[0])
     out = _out(call, out, q, "out")
-    lse = call.empty(q.shape[:3], N.LC_DTYPE_F32) if return_lse else None
-    tq, tk, tv, to = (_tensor4(call, x, n) for x, n in ((q, "q"), (k, "k"), (v, "v"), (out, "out")))
+    lse = call.empty(q, q.shape[:3], N.LC_DTYPE_F32) if return_lse else None
+    ws = call.workspace(nbytes)
     _check(_lib().lcCrossAttentionForward(
-        _byref(cfg), _byref(tq), _byref(tk), _byref(tv), None if lengths is None else call.addr(lengths), _byref(to),
-        None if lse is None else call.addr(lse), call.workspace(nbytes), nbytes, call.stream))
+        cfg, _tensor4(call, q, "q"), _tensor4(call, k, "k"), _tensor4(call, v, "v"), _addr(call, lengths),
+        _tensor4(call, out, "out"), _addr(call, lse), _addr(call, ws), nbytes, call.stream))
     got = call.finish(out, lse)
     return got if return_lse else got[0]
 
@@ -356,21 +382,20 @@ def cross_attention_backward(dout, q, k, v, out, lse, kv_lengths=None, *, scale=
         raise ValueError("lse must be contiguous float32")
     lengths = _lengths(call, kv_lengths, q.shape[0])
     dq, dk, dv = call.empty_like(q), call.empty_like(k), call.empty_like(v)
-    t = [_tensor4(call, x, n) for x, n in ((dout, "dout"), (q, "q"), (k, "k"), (v, "v"), (out, "out"), (dq, "dq"),
-                                           (dk, "dk"), (dv, "dv"))]
-    t = [_byref(x) for x in t]
+    ws = call.workspace(nbytes)
     _check(_lib().lcCrossAttentionBackward(
-        _byref(cfg), t[0], t[1], t[2], t[3], t[4], call.addr(lse), None if lengths is None else call.addr(lengths),
-        t[5], t[6], t[7], call.workspace(nbytes), nbytes, call.stream))
+        cfg, _tensor4(call, dout, "dout"), _tensor4(call, q, "q"), _tensor4(call, k, "k"), _tensor4(call, v, "v"),
+        _tensor4(call, out, "out"), call.addr(lse), _addr(call, lengths), _tensor4(call, dq, "dq"),
+        _tensor4(call, dk, "dk"), _tensor4(call, dv, "dv"), _addr(call, ws), nbytes, call.stream))
     return call.finish(dq, dk, dv)
 
 
 @functools.lru_cache(maxsize=512)
 def _ln_plan(*key):
-    cfg = N.LayerNormConfig(*key)
+    cfg = N.LayerNormConfig(*key, 1)
     n = ctypes.c_size_t()
     _check(_lib().lcLayerNormWorkspaceSize(_byref(cfg), _byref(n)))
-    return cfg, n.value
+    return _byref(cfg), n.value
 
 
 def _vector(call, x, n, dtype, name):
@@ -414,14 +439,13 @@ def layer_norm(x, weight=None, bias=None, *, eps=1e-5, return_stats=False):
             raise ValueError("weight and bias must have one type")
         wd = bd
     cfg, _ = _ln_plan(rows, n, dtype, dtype if wd is None else wd, float(eps))
-    y = call.empty(x.shape, dtype)
+    y = call.empty_contiguous(x)
     mean = rstd = None
     if return_stats:
-        mean, rstd = call.empty(x.shape[:-1], N.LC_DTYPE_F32), call.empty(x.shape[:-1], N.LC_DTYPE_F32)
-    a = call.addr
+        mean, rstd = call.empty(x, x.shape[:-1], N.LC_DTYPE_F32), call.empty(x, x.shape[:-1], N.LC_DTYPE_F32)
     _check(_lib().lcLayerNormForward(
-        _byref(cfg), a(x), stride, None if weight is None else a(weight), None if bias is None else a(bias), a(y), n,
-        None if mean is None else a(mean), None if rstd is None else a(rstd), call.stream))
+        cfg, call.addr(x), stride, _addr(call, weight), _addr(call, bias), call.addr(y), n, _addr(call, mean),
+        _addr(call, rstd), call.stream))
     got = call.finish(y, mean, rstd)
     return got if return_stats else got[0]
 
@@ -448,14 +472,14 @@ def layer_norm_backward(dy, x, weight, mean, rstd):
         if call.dtype(s, name) != N.LC_DTYPE_F32 or not call.is_contiguous(s):
             raise ValueError(f"{name} must be contiguous float32")
     cfg, nbytes = _ln_plan(rows, n, dtype, wd, 0.0)
-    dx = call.empty(x.shape, dtype)
+    dx = call.empty_contiguous(x)
     dw = db = None
     if weight is not None:
-        dw, db = call.empty((n,), wd), call.empty((n,), wd)
-    a = call.addr
+        dw, db = call.empty_contiguous(weight), call.empty_contiguous(weight)
+    ws = call.workspace(nbytes)
     _check(_lib().lcLayerNormBackward(
-        _byref(cfg), a(dy), dy_stride, a(x), stride, None if weight is None else a(weight), a(mean), a(rstd), a(dx), n,
-        None if dw is None else a(dw), None if db is None else a(db), call.workspace(nbytes), nbytes, call.stream))
+        cfg, call.addr(dy), dy_stride, call.addr(x), stride, _addr(call, weight), call.addr(mean), call.addr(rstd),
+        call.addr(dx), n, _addr(call, dw), _addr(call, db), _addr(call, ws), nbytes, call.stream))
     return call.finish(dx, dw, db)
 
 
@@ -469,7 +493,7 @@ def _cache(call, k_pages, v_pages, k_scales, v_scales):
     _same(vp, (pages, heads, d, KV_PAGE_TOKENS), "v_pages")
     _same(ks, (pages, heads), "k_scales")
     _same(vs, (pages, heads), "v_scales")
-    return N.KvCache(call.addr(kp), call.addr(vp), call.addr(ks), call.addr(vs), pages, heads, d), (kp, vp, ks, vs)
+    return N.KvCache(call.addr(kp), call.addr(vp), call.addr(ks), call.addr(vs), pages, heads, d, 1), (kp, vp, ks, vs)
 
 
 def _table(call, block_table, batch):
@@ -507,11 +531,20 @@ def kv_cache_store(k, v, block_table, kv_lengths, k_pages, v_pages, k_scales, v_
         raise ValueError("k and the cache must agree in kv_heads and head_dim")
     lengths = _lengths(call, kv_lengths, b)
     t, stride = _table(call, block_table, b)
-    tk, tv = _tensor4(call, k, "k"), _tensor4(call, v, "v")
     _check(_lib().lcKvCacheStore(
-        _byref(c), b, sk, call.dtype(k, "k"), _byref(tk), _byref(tv), call.addr(t), t.shape[1], stride,
-        None if lengths is None else call.addr(lengths), call.stream))
+        _byref(c), b, sk, call.dtype(k, "k"), _tensor4(call, k, "k"), _tensor4(call, v, "v"), call.addr(t), t.shape[1],
+        stride, _addr(call, lengths), call.stream))
     call.finish(*pool)
+
+
+@functools.lru_cache(maxsize=1024)
+def _kv_plan(pages, kv_heads, d, b, hq, sq, width, dtype, scale):
+    # The size does not depend on where the pool lies: any aligned base does.
+    cache = N.KvCache(16, 16, 16, 16, pages, kv_heads, d)
+    cfg = N.KvAttentionConfig(b, hq, sq, width, dtype, scale)
+    n = ctypes.c_size_t()
+    _check(_lib().lcKvCacheAttentionWorkspaceSize(_byref(cache), _byref(cfg), _byref(n)))
+    return _byref(cfg), n.value
 
 
 def kv_cache_attention(q, k_pages, v_pages, k_scales, v_scales, block_table, kv_lengths=None, *, scale=None,
@@ -535,14 +568,12 @@ def kv_cache_attention(q, k_pages, v_pages, k_scales, v_scales, block_table, kv_
         raise ValueError("q's heads must be a multiple of the cache's")
     lengths = _lengths(call, kv_lengths, b)
     t, stride = _table(call, block_table, b)
-    cfg = N.KvAttentionConfig(b, hq, sq, t.shape[1], call.dtype(q, "q"), _scale(scale))
-    need = ctypes.c_size_t()
-    _check(_lib().lcKvCacheAttentionWorkspaceSize(_byref(c), _byref(cfg), _byref(need)))
+    cfg, nbytes = _kv_plan(c.pages, c.kv_heads, d, b, hq, sq, t.shape[1], call.dtype(q, "q"), _scale(scale))
     out = _out(call, out, q, "out")
-    lse = call.empty(q.shape[:3], N.LC_DTYPE_F32) if return_lse else None
-    tq, to = _tensor4(call, q, "q"), _tensor4(call, out, "out")
+    lse = call.empty(q, q.shape[:3], N.LC_DTYPE_F32) if return_lse else None
+    ws = call.workspace(nbytes)
     _check(_lib().lcKvCacheAttention(
-        _byref(c), _byref(cfg), _byref(tq), call.addr(t), stride, None if lengths is None else call.addr(lengths),
-        _byref(to), None if lse is None else call.addr(lse), call.workspace(need.value), need.value, call.stream))
+        _byref(c), cfg, _tensor4(call, q, "q"), call.addr(t), stride, _addr(call, lengths), _tensor4(call, out, "out"),
+        _addr(call, lse), _addr(call, ws), nbytes, call.stream))
     got = call.finish(out, lse)
     return got if return_lse else got[0]

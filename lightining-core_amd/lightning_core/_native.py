@@ -124,16 +124,17 @@ class DeviceTensor(ctypes.Structure):
 
 class CrossAttentionConfig(ctypes.Structure):
     _fields_ = [("batch", c_size), ("heads", c_size), ("kv_heads", c_size), ("q_len", c_size), ("kv_len", c_size),
-                ("head_dim", c_size), ("dtype", c_int), ("scale", c_float)]
+                ("head_dim", c_size), ("dtype", c_int), ("scale", c_float), ("trusted_pointers", c_int)]
 
 
 class LayerNormConfig(ctypes.Structure):
-    _fields_ = [("rows", c_size), ("n", c_size), ("dtype", c_int), ("weight_dtype", c_int), ("eps", c_float)]
+    _fields_ = [("rows", c_size), ("n", c_size), ("dtype", c_int), ("weight_dtype", c_int), ("eps", c_float),
+                ("trusted_pointers", c_int)]
 
 
 class KvCache(ctypes.Structure):
     _fields_ = [("k_pages", c_void_p), ("v_pages", c_void_p), ("k_scales", c_void_p), ("v_scales", c_void_p),
-                ("pages", c_size), ("kv_heads", c_size), ("head_dim", c_size)]
+                ("pages", c_size), ("kv_heads", c_size), ("head_dim", c_size), ("trusted_pointers", c_int)]
 
 
 class KvAttentionConfig(ctypes.Structure):
@@ -237,6 +238,7 @@ SIGNATURES = {
     "lcVitBlockSessionForward": (_E, [c_void_p, BUF, BUF]),
     "lcVitBlockSessionRunCached": (_E, [c_void_p, c_size]),
     "lcVitBlockForward": (_E, [BUF, BUF, BUF, BUF, BUF, P(VitBlockConfig), c_int]),
+    "lcHipDeviceIndex": (_E, [P(c_int)]),
     "lcHipBackendStream": (_E, [P(c_void_p)]),
     "lcCrossAttentionWorkspaceSize": (_E, [P(CrossAttentionConfig), c_int, P(c_size)]),
     "lcCrossAttentionForward": (_E, [P(CrossAttentionConfig)] + [P(DeviceTensor)] * 3 + [BUF, P(DeviceTensor), BUF, BUF,

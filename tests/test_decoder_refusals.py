@@ -34,7 +34,7 @@ def test_cross_attention_configurations(change, status):
 
 def test_cross_attention_workspace():
     # few row blocks: the keys are split, and each split keeps a row and two statistics
-    st, n = _size(_cfg(b=1, h=12, hkv=12, sq=1, sk=196))
+    st, n = _size(_cfg(b=1, h=12, hkv=12, sq=1, sk=30000))
     assert st == 0 and n > 0 and n % (12 * (64 + 2) * 4) == 0
     assert _size(_cfg(b=64, h=16, hkv=16, sq=200, sk=4096)) == (0, 0)  # enough of them
     st, n = _size(_cfg(b=64, h=16, hkv=16, sq=200, sk=4096), 1)
