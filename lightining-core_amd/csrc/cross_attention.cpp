@@ -10,15 +10,25 @@ namespace {
 
 constexpr const char* kOp = "cross attention";
 constexpr std::size_t kMostRows = std::size_t{1} << 30;
-// Workgroups that fill the chip (256 CUs, two each).  A split beyond that only
-// adds partial results to join.
-constexpr std::size_t kTarget = 512;
+// Workgroups that run at once on 256 CUs: two a CU, of the few-row forward one.
+constexpr std::size_t kSlots = 512;
+constexpr std::size_t kFewSlots = 256;
 // Up to so many query rows of a problem, the forward's waves share the keys
-// instead of the rows (one workgroup on a CU).
+// instead of the rows.
 constexpr std::size_t kFewRows = 64;
-constexpr std::size_t kFewTarget = 256;
+// A workgroup's start and end, and a join, in tiles' time (splitCount).
+constexpr double kFixed = 2.0;
+constexpr double kJoin = 3.0;
+// The backward pass's work is counted in products of 32 x 32 blocks: dQ has three
+// for a block, dK and dV four.  A workgroup gets at most kShare of what each
+// place on the chip has to do in all, so that the short ones fill what the long
+// ones leave, and no less than kLeast, below which its start and its partial
+// result cost more than its work.
+constexpr double kShare = 0.8;
+constexpr std::size_t kMostShares = 32;
+constexpr double kLeast = 8.0;
 
-// How the three kernels share the work of a problem, and the workspace that it
+// How the kernels share the work of a problem, and the workspace that it
 // takes: a function of the shape alone, so that the size a caller asks for is
 // the one its call needs.
 struct Plan {
@@ -30,12 +40,11 @@ struct Plan {
     return splits_fwd > 1 ? static_cast<std::size_t>(splits_fwd) * rows_q * (width + 2) * sizeof(float) : 0;
   }
   std::size_t deltaBytes() const { return roundUp(rows_q * 2 * sizeof(float), 256); }
-  // The partial gradients of Q, then (they are joined by then) of K and V.
-  std::size_t backwardBytes() const {
-    const std::size_t q = splits_q > 1 ? static_cast<std::size_t>(splits_q) * rows_q * width : 0;
-    const std::size_t kv = splits_kv > 1 ? static_cast<std::size_t>(splits_kv) * 2 * rows_kv * width : 0;
-    return deltaBytes() + std::max(q, kv) * sizeof(float);
+  std::size_t partialQ() const { return splits_q > 1 ? static_cast<std::size_t>(splits_q) * rows_q * width : 0; }
+  std::size_t partialKv() const {
+    return splits_kv > 1 ? static_cast<std::size_t>(splits_kv) * 2 * rows_kv * width : 0;
   }
+  std::size_t backwardBytes() const { return deltaBytes() + (partialQ() + partialKv()) * sizeof(float); }
 };
 
 Plan planOf(const lcCrossAttentionConfig& c) {
@@ -52,12 +61,21 @@ Plan planOf(const lcCrossAttentionConfig& c) {
   const std::size_t few_rows = kern::kXAttnFewRows;
   p.few = group * c.q_len <= kFewRows;
   p.splits_fwd = p.few ? splitCount(problems * ((group * c.q_len + few_rows - 1) / few_rows), (kv_tiles + 3) / 4,
-                                    kFewTarget)
-                       : splitCount(q_blocks, kv_tiles, kTarget);
-  p.splits_q = splitCount(q_blocks, kv_tiles, kTarget);
+                                    kFewSlots, kFixed, kJoin)
+                       : splitCount(q_blocks, kv_tiles, kSlots, kFixed, kJoin);
   const std::size_t q_tile = kern::kXAttnQueryTile;
-  p.splits_kv = splitCount(problems * ((c.kv_len + block - 1) / block), group * ((c.q_len + q_tile - 1) / q_tile),
-                           kTarget);
+  const std::size_t kv_blocks = problems * ((c.kv_len + block - 1) / block);
+  const std::size_t q_tiles = group * ((c.q_len + q_tile - 1) / q_tile);
+  const double work_q = 3.0 * static_cast<double>(tile / 32 * kv_tiles);  // of one block
+  const double work_kv = 4.0 * static_cast<double>(q_tiles);
+  const double all = work_q * static_cast<double>(q_blocks) + work_kv * static_cast<double>(kv_blocks);
+  const double most = std::max(kLeast, kShare * all / static_cast<double>(kSlots));
+  const auto shares = [most](double work, std::size_t tiles) {
+    const std::size_t want = static_cast<std::size_t>(std::ceil(work / most));
+    return static_cast<int>(std::max<std::size_t>(1, std::min({want, tiles, kMostShares})));
+  };
+  p.splits_q = shares(work_q, kv_tiles);
+  p.splits_kv = shares(work_kv, q_tiles);
   return p;
 }
 
@@ -83,8 +101,8 @@ Status checkConfig(const lcCrossAttentionConfig* c) {
   // Row indices and grids are 32-bit.
   const std::size_t most = kMostRows;
   if (c->batch > most || c->heads > most || c->q_len > most || c->kv_len > most ||
-      c->batch * c->kv_heads > most || (c->heads / c->kv_heads) * c->q_len > most / 256 ||
-      c->kv_len > most / 256) {
+      c->batch * c->kv_heads > most || (c->heads / c->kv_heads) * c->q_len > most / 512 ||
+      c->kv_len > most / 512) {
     return fail(Status::kNotSupported, "cross attention: shape too large");
   }
   return Status::kSuccess;
@@ -152,7 +170,7 @@ Status forward(const lcCrossAttentionConfig* cfg, const lcDeviceTensor* q, const
   }
   traceOpDispatch(TraceOp::kAttentionForward, Device::kHIP, Device::kHIP, false, c.q_len * c.kv_len * c.head_dim);
   const hipStream_t s = static_cast<hipStream_t>(stream);
-  LC_HIP_TRY(kern::crossAttention(kern::XAttnStep::kForward, a, dtypeOf(c.dtype), aligned, s));
+  LC_HIP_TRY(kern::crossAttentionForward(a, dtypeOf(c.dtype), aligned, s));
   if (a.splits > 1) {
     LC_HIP_TRY(kern::crossAttentionJoin(a, dtypeOf(c.dtype), s));
   }
@@ -196,23 +214,11 @@ Status backward(const lcCrossAttentionConfig* cfg, const lcDeviceTensor* dout, c
   a.lse = const_cast<float*>(lse);
   a.lengths = kv_lengths;
   a.delta = static_cast<float*>(workspace);
-  a.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + plan.deltaBytes());
-  const hipStream_t s = static_cast<hipStream_t>(stream);
-  const kern::DType type = dtypeOf(c.dtype);
-  if (plan.rows_q != 0) {
-    a.splits = plan.splits_q;
-    LC_HIP_TRY(kern::crossAttention(kern::XAttnStep::kGradQ, a, type, aligned, s));
-    if (a.splits > 1) {
-      LC_HIP_TRY(kern::crossAttentionSum(a.part, a.dq, nullptr, a.splits, a.batch, a.heads, a.q_len, a.d, type, s));
-    }
-  }
-  if (plan.rows_kv != 0) {
-    a.splits = plan.splits_kv;
-    LC_HIP_TRY(kern::crossAttention(kern::XAttnStep::kGradKV, a, type, aligned, s));
-    if (a.splits > 1) {
-      LC_HIP_TRY(kern::crossAttentionSum(a.part, a.dk, &a.dv, a.splits, a.batch, a.kv_heads, a.kv_len, a.d, type, s));
-    }
-  }
+  a.part_q = reinterpret_cast<float*>(static_cast<char*>(workspace) + plan.deltaBytes());
+  a.part_kv = a.part_q + plan.partialQ();
+  a.splits_q = plan.splits_q;
+  a.splits_kv = plan.splits_kv;
+  LC_HIP_TRY(kern::crossAttentionBackward(a, dtypeOf(c.dtype), aligned, static_cast<hipStream_t>(stream)));
   return Status::kSuccess;
 }
 

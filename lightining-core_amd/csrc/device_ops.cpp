@@ -82,11 +82,26 @@ Status takeTensor(const char* op, const char* name, const lcDeviceTensor* t, std
   return Status::kSuccess;
 }
 
-int splitCount(std::size_t blocks, std::size_t tiles, std::size_t target) {
-  if (blocks == 0 || tiles <= 1 || blocks >= target) {
+int splitCount(std::size_t blocks, std::size_t tiles, std::size_t slots, double fixed, double join) {
+  if (blocks == 0 || tiles <= 1) {
     return 1;
   }
-  return static_cast<int>(std::min(tiles, (target + blocks - 1) / blocks));
+  int best = 1;
+  double least = 0.0;
+  const std::size_t most = std::min<std::size_t>(tiles, 32);
+  for (std::size_t s = 1; s <= most; ++s) {
+    const std::size_t share = (tiles + s - 1) / s;
+    if (s > 1 && share == (tiles + s - 2) / (s - 1)) {
+      continue;  // no shorter than with one share less
+    }
+    const double rounds = static_cast<double>((blocks * s + slots - 1) / slots);
+    const double cost = rounds * (static_cast<double>(share) + fixed) + (s > 1 ? join : 0.0);
+    if (s == 1 || cost < least) {
+      least = cost;
+      best = static_cast<int>(s);
+    }
+  }
+  return best;
 }
 
 }  // namespace lchip

@@ -45,7 +45,11 @@ Status takeTensor(const char* op, const char* name, const lcDeviceTensor* t, std
                   std::size_t rows, std::size_t d, lcDataType type, bool written, kern::XTensor* out, bool* aligned);
 
 // The workgroups that should share the tiles of one row block, when `blocks` of
-// them are there and each has `tiles`.
-int splitCount(std::size_t blocks, std::size_t tiles, std::size_t target);
+// them are there, each has `tiles` and the chip runs `slots` workgroups at once.
+// A workgroup's time is its tiles plus `fixed` (its start and its end, in tiles);
+// the chip's is that times the rounds of workgroups, and a last round that is
+// nearly empty costs as much as a full one.  The join of more than one share
+// costs `join` tiles.  At most 32 shares.
+int splitCount(std::size_t blocks, std::size_t tiles, std::size_t slots, double fixed, double join);
 
 }  // namespace lchip

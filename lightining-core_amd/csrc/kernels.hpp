@@ -352,10 +352,19 @@ struct XAttnArgs {
   float c;      // |scale| * log2(e); `negate` when scale < 0
   float scale;
   int negate;
-  int splits;    // workgroups that share a row block's tiles
-  int few;       // forward: blocks of kXAttnFewRows rows, waves that share the keys
+  // Forward.  few: blocks of kXAttnFewRows rows, waves that share the keys;
+  // splits: workgroups that share a row block's tiles, joined by
+  // crossAttentionJoin.
+  int few;
+  int splits;
   float* part;   // splits > 1: [splits][rows][kXAttnWidth(d)]
-  float* stats;  // splits > 1, forward: [splits][rows][2]
+  float* stats;  // splits > 1: [splits][rows][2]
+  // Backward: the shares of a row block's key tiles and of a key block's query
+  // tiles, and where more than one put their partial gradients:
+  // [splits_q][rows][width], [splits_kv][2][rows][width].
+  int splits_q, splits_kv;
+  float* part_q;
+  float* part_kv;
 };
 constexpr int kXAttnRows = 128;  // rows (or keys) of a workgroup
 constexpr int kXAttnMaxDim = 128;
@@ -363,15 +372,12 @@ constexpr int kXAttnWidth(int d) { return d <= 64 ? 64 : 128; }
 constexpr int kXAttnFewRows = 32;
 constexpr int kXAttnTile(DType t) { return t == DType::kF32 ? 32 : 64; }  // keys
 constexpr int kXAttnQueryTile = 32;                                       // queries, for dK and dV
-enum class XAttnStep { kForward, kGradQ, kGradKV };
-// One kernel of the set.  `aligned`: every tensor's base is 16-byte aligned, its
-// strides and d are multiples of 16 bytes.
-hipError_t crossAttention(XAttnStep step, const XAttnArgs& a, DType type, bool aligned, hipStream_t stream);
-// Joins the forward's splits; sums the backward's (x, then `second`, each
-// [batch, heads, len, d], from part [splits][1 or 2][batch * heads * len][width]).
+// `aligned`: every tensor's base is 16-byte aligned, its strides and d are
+// multiples of 16 bytes.
+hipError_t crossAttentionForward(const XAttnArgs& a, DType type, bool aligned, hipStream_t stream);
 hipError_t crossAttentionJoin(const XAttnArgs& a, DType type, hipStream_t stream);
-hipError_t crossAttentionSum(const float* part, const XTensor& x, const XTensor* second, int splits, int batch,
-                             int heads, int len, int d, DType type, hipStream_t stream);
+// The whole backward pass (no rows of one side or the other are fine).
+hipError_t crossAttentionBackward(const XAttnArgs& a, DType type, bool aligned, hipStream_t stream);
 
 // ---- layer norm (layer_norm.hip) ----------------------------------------------
 // Rows of n values with row strides in elements.  Forward: x -> y (mean and

@@ -3,7 +3,7 @@
 //
 // One problem is a (batch row, key/value head) pair: the `group` query heads
 // that share the head give R = group * q_len rows, against the row's own
-// number of keys.  All three kernels have one shape: a wave owns 32 rows of
+// number of keys.  All three parts have one shape: a wave owns 32 rows of
 // one side (queries for O and dQ, keys for dK and dV), one per MFMA column, and
 // the other side streams through LDS in tiles.  Scores are computed with the
 // streamed side as MFMA rows, so a lane holds scores of its own row only, and
@@ -14,9 +14,10 @@
 //   dQ       S^T = K Q^T, dP^T = V dO^T, dQ^T += K^T dS^T
 //   dK, dV   S = Q K^T, dP = dO V^T, dV^T += dO^T P, dK^T += Q^T dS
 // with P = exp(scale S - lse), dS = P o (dP - delta), delta = rowsum(dO o O).
-// The two backward kernels compute the scores twice (14 products of the
-// algorithm's 10) so that every gradient has one writer: no atomics, the same
-// bits every time.
+// The backward pass computes the scores twice (14 products of the algorithm's
+// 10) so that every gradient has one writer: no atomics, the same bits every
+// time.  dQ and dK / dV are different workgroups of one launch, so that the one
+// fills the chip where the other has too few.
 #include <hip/hip_runtime.h>
 
 #include "../kernels.hpp"
@@ -27,7 +28,6 @@ namespace lchip::k {
 namespace {
 
 using kern::XAttnArgs;
-using kern::XAttnStep;
 using kern::XTensor;
 
 constexpr float kLog2e = 1.4426950408889634f;
@@ -752,16 +752,52 @@ __device__ __forceinline__ int exponent_of(float amax) {
 }
 __device__ __forceinline__ float power_of_two(int e) { return __builtin_amdgcn_ldexpf(1.0f, e); }
 
-// dQ: as the forward, with dO's rows beside Q's.  Writes each query row's delta
-// (and, for fp16, the exponent of its dO) for the dK / dV kernel.
+// Each query row's delta = dO . O and the exponent of its dO, 16 threads a row.
+template <typename T, bool VEC>
+__global__ __launch_bounds__(256) void xattn_delta_kernel(XAttnArgs a) {
+  using E = typename Elem<T>::type;
+  constexpr int EC = Elem<T>::kChunk;
+  const size_t rows = static_cast<size_t>(a.batch) * a.heads * a.q_len;
+  const size_t row = static_cast<size_t>(blockIdx.x) * 16 + (threadIdx.x >> 4);
+  const size_t at = row < rows ? row : 0;
+  const size_t head = at / a.q_len;
+  const int64_t pos = static_cast<int64_t>(at - head * a.q_len);
+  const int64_t b = static_cast<int64_t>(head / a.heads);
+  const int64_t h = static_cast<int64_t>(head - b * a.heads);
+  const E* g = static_cast<const E*>(a.go.p) + b * a.go.sb + h * a.go.sh + pos * a.go.ss;
+  const E* o = static_cast<const E*>(a.o.p) + b * a.o.sb + h * a.o.sh + pos * a.o.ss;
+  float delta = 0.0f;
+  float amax = 0.0f;
+#pragma unroll
+  for (int j = 0; j < kern::kXAttnMaxDim / (16 * EC); ++j) {
+    const int c = (threadIdx.x & 15) + 16 * j;
+    const u32x4 gv = load_chunk<T, VEC>(g, c, a.d);
+    const u32x4 ov = load_chunk<T, VEC>(o, c, a.d);
+#pragma unroll
+    for (int i = 0; i < EC; ++i) {
+      delta = fmaf(chunk_value<T>(gv, i), chunk_value<T>(ov, i), delta);
+      amax = fmaxf(amax, fabsf(chunk_value<T>(gv, i)));
+    }
+  }
+#pragma unroll
+  for (int x = 8; x > 0; x >>= 1) {
+    delta += __shfl_xor(delta, x);
+    amax = fmaxf(amax, __shfl_xor(amax, x));
+  }
+  if ((threadIdx.x & 15) == 0 && row < rows) {
+    *reinterpret_cast<float2*>(a.delta + 2 * row) = make_float2(delta, static_cast<float>(exponent_of(amax)));
+  }
+}
+
+// dQ of 128 rows (block `blk`) over share z of the keys: as the forward, with
+// dO's rows beside Q's.
 template <typename T, int DP, bool VEC>
-__global__ __launch_bounds__(256, (waves_per_simd<T, DP, VEC>())) void xattn_dq_kernel(XAttnArgs a) {
+__device__ __forceinline__ void dq_part(const XAttnArgs& a, char* smem, int blk, int z) {
   using TL = Tile<T, DP>;
   using E = typename Elem<T>::type;
   constexpr int KT = tile_keys<T>();
   constexpr int NB = KT / 32;
   constexpr int TB = KT * TL::RB;
-  extern __shared__ __attribute__((aligned(16))) char smem[];
   const int tid = threadIdx.x;
   const int lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -770,12 +806,12 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP, VEC>())) void xattn_dq_
   const int hk = blockIdx.x - b * a.kv_heads;
   const int group = a.heads / a.kv_heads;
   const int R = group * a.q_len;
-  const int r = blockIdx.y * 128 + wave * 32 + (lane & 31);
+  const int r = blk * 128 + wave * 32 + (lane & 31);
   const bool valid = r < R;
   const QueryRow qr = query_row(valid ? r : 0, a.q_len, hk * group);
   const int len = keys_of(a, b);
   int t0, t1;
-  tile_range((len + KT - 1) / KT, a.splits, blockIdx.z, &t0, &t1);
+  tile_range((len + KT - 1) / KT, a.splits_q, z, &t0, &t1);
 
   Stream<T, DP, KT, VEC, 4> ks, vs;
   ks.init(static_cast<const E*>(a.k.p) + b * a.k.sb + hk * a.k.sh, a.k.ss, len, a.d, wave, lane);
@@ -788,23 +824,6 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP, VEC>())) void xattn_dq_
   u32x4 qf[TL::NS], gf[TL::NS];
   load_fragments<T, DP, VEC>(static_cast<const E*>(a.go.p) + b * a.go.sb + qr.head * a.go.sh + pos * a.go.ss, valid,
                              a.d, half, gf);
-  float delta = 0.0f;
-  float amax = 0.0f;
-  {
-    load_fragments<T, DP, VEC>(static_cast<const E*>(a.o.p) + b * a.o.sb + qr.head * a.o.sh + pos * a.o.ss, valid, a.d,
-                               half, qf);
-#pragma unroll
-    for (int s = 0; s < TL::NS; ++s) {
-#pragma unroll
-      for (int i = 0; i < TL::EC; ++i) {
-        const float g = chunk_value<T>(gf[s], i);
-        delta = fmaf(g, chunk_value<T>(qf[s], i), delta);
-        amax = fmaxf(amax, fabsf(g));
-      }
-    }
-    delta = add_xor32(delta);
-    amax = max_xor32(amax);
-  }
   load_fragments<T, DP, VEC>(static_cast<const E*>(a.q.p) + b * a.q.sb + qr.head * a.q.sh + pos * a.q.ss, valid, a.d,
                              half, qf);
   if (a.negate) {
@@ -815,11 +834,9 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP, VEC>())) void xattn_dq_
   }
   const size_t lrow = (static_cast<size_t>(b) * a.heads + qr.head) * a.q_len + qr.pos;
   const float lse2 = valid ? a.lse[lrow] * kLog2e : 0.0f;
-  const int ex = exponent_of(amax);
-  if (valid && half == 0 && blockIdx.z == 0) {
-    a.delta[2 * lrow] = delta;
-    a.delta[2 * lrow + 1] = static_cast<float>(ex);
-  }
+  const float2 de = valid ? *reinterpret_cast<const float2*>(a.delta + 2 * lrow) : make_float2(0.0f, 0.0f);
+  const float delta = de.x;
+  const int ex = static_cast<int>(de.y);
   float down = 1.0f;
   if constexpr (__is_same(T, F16)) {
     down = power_of_two(-ex);
@@ -884,9 +901,9 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP, VEC>())) void xattn_dq_
   if constexpr (__is_same(T, F16)) {
     f *= power_of_two(ex);
   }
-  if (a.splits > 1) {
-    const size_t prow = (static_cast<size_t>(blockIdx.z) * gridDim.x + blockIdx.x) * R + r;
-    store_partial<TL::DT>(a.part + prow * DP, half, dq, f);
+  if (a.splits_q > 1) {
+    const size_t prow = (static_cast<size_t>(z) * gridDim.x + blockIdx.x) * R + r;
+    store_partial<TL::DT>(a.part_q + prow * DP, half, dq, f);
     return;
   }
   store_column<T, TL::DT, VEC>(static_cast<E*>(a.dq.p) + b * a.dq.sb + qr.head * a.dq.sh + pos * a.dq.ss, a.d, half,
@@ -899,18 +916,18 @@ constexpr size_t dkv_lds_bytes() {
   return (4 * kQueryTile + 128) * Tile<T, DP>::RB + 6 * kQueryTile * sizeof(float);
 }
 
-// dK and dV: grid (problems, 128-key blocks, splits of the query tiles), four
-// waves of 32 keys; Q and dO stream.  The workgroup's own rows of V stay in LDS:
-// in registers beside K's and two accumulators they would leave room for one
-// wave on a SIMD, whose products then wait for its exponentials (16-bit, 64
-// heads of 2048 x 1500 x 128: 465 us).
+// dK and dV of 128 keys (block `blk`), four waves of 32, over share z of the
+// query tiles; Q and dO stream.  The workgroup's own rows of V stay in LDS: in
+// registers beside K's and two accumulators they would leave room for one wave
+// on a SIMD, whose products then wait for its exponentials (16-bit, 64 heads of
+// 2048 x 1500 x 128: 465 us against 358).
 template <typename T, int DP, bool VEC>
-__global__ __launch_bounds__(256, (VEC && Elem<T>::kChunk == 8 ? 2 : 1)) void xattn_dkv_kernel(XAttnArgs a) {
+__device__ __forceinline__ void dkv_part(const XAttnArgs& a, char* smem, int blk, int z) {
   using TL = Tile<T, DP>;
   using E = typename Elem<T>::type;
   constexpr int KT = kQueryTile;
   constexpr int TB = KT * TL::RB;
-  extern __shared__ __attribute__((aligned(16))) char smem[];  // Q, dO tiles, lse, delta and exponents, V
+  // LDS: Q and dO tiles, then lse, delta and exponents, then V.
   float* const st = reinterpret_cast<float*>(smem + 4 * TB);   // [2][3][KT]
   char* const own = smem + 4 * TB + 6 * KT * sizeof(float);
   const int tid = threadIdx.x;
@@ -920,13 +937,13 @@ __global__ __launch_bounds__(256, (VEC && Elem<T>::kChunk == 8 ? 2 : 1)) void xa
   const int b = blockIdx.x / a.kv_heads;
   const int hk = blockIdx.x - b * a.kv_heads;
   const int group = a.heads / a.kv_heads;
-  const int key = blockIdx.y * 128 + wave * 32 + (lane & 31);
+  const int key = blk * 128 + wave * 32 + (lane & 31);
   const int len = keys_of(a, b);
   const bool valid = key < len;
   // Tiles: those of the group's heads, one after the other.
   const int per_head = (a.q_len + KT - 1) / KT;
   int t0, t1;
-  tile_range(static_cast<int>(blockIdx.y) * 128 < len ? group * per_head : 0, a.splits, blockIdx.z, &t0, &t1);
+  tile_range(blk * 128 < len ? group * per_head : 0, a.splits_kv, z, &t0, &t1);
 
   Stream<T, DP, KT, VEC, 4> qs, gs;
   float rl = 0.0f, rd = 0.0f, re = 0.0f;
@@ -965,7 +982,7 @@ __global__ __launch_bounds__(256, (VEC && Elem<T>::kChunk == 8 ? 2 : 1)) void xa
     stage(t0, 0);
     Stream<T, DP, 128, VEC, 4> vs;
     vs.init(vbase, a.v.ss, len, a.d, wave, lane);
-    vs.stage(blockIdx.y, own);
+    vs.stage(blk, own);
   }
   load_fragments<T, DP, VEC>(static_cast<const E*>(a.k.p) + b * a.k.sb + hk * a.k.sh + krow * a.k.ss, valid, a.d, half,
                              kf);
@@ -1068,11 +1085,11 @@ __global__ __launch_bounds__(256, (VEC && Elem<T>::kChunk == 8 ? 2 : 1)) void xa
       dv[t] = zero16();
     }
   }
-  if (a.splits > 1) {
+  if (a.splits_kv > 1) {
     const size_t plane = static_cast<size_t>(gridDim.x) * a.kv_len;
-    const size_t prow = static_cast<size_t>(blockIdx.z) * 2 * plane + static_cast<size_t>(blockIdx.x) * a.kv_len + key;
-    store_partial<TL::DT>(a.part + prow * DP, half, dk, fk);
-    store_partial<TL::DT>(a.part + (prow + plane) * DP, half, dv, fv);
+    const size_t prow = static_cast<size_t>(z) * 2 * plane + static_cast<size_t>(blockIdx.x) * a.kv_len + key;
+    store_partial<TL::DT>(a.part_kv + prow * DP, half, dk, fk);
+    store_partial<TL::DT>(a.part_kv + (prow + plane) * DP, half, dv, fv);
     return;
   }
   const int64_t at = key;
@@ -1080,15 +1097,35 @@ __global__ __launch_bounds__(256, (VEC && Elem<T>::kChunk == 8 ? 2 : 1)) void xa
   store_column<T, TL::DT, VEC>(static_cast<E*>(a.dv.p) + b * a.dv.sb + hk * a.dv.sh + at * a.dv.ss, a.d, half, dv, fv);
 }
 
-// Sums the splits' partial rows [splits][planes][rows][DP] in split order into
-// strided [batch, heads, len, d] tensors, one per plane: a wave per row.
+// The whole backward pass: grid (problems, workgroups), the dK / dV ones (the
+// longer ones) first.
+template <typename T, int DP, bool VEC>
+__global__ __launch_bounds__(256, (VEC && (Elem<T>::kChunk == 8 || DP == 64) ? 2 : 1)) void xattn_bwd_kernel(
+    XAttnArgs a) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const int kv_blocks = (a.kv_len + 127) / 128;
+  const int y = blockIdx.y;
+  if (y < kv_blocks * a.splits_kv) {
+    dkv_part<T, DP, VEC>(a, smem, y % kv_blocks, y / kv_blocks);
+  } else {
+    const int q_blocks = (a.heads / a.kv_heads * a.q_len + 127) / 128;
+    const int i = y - kv_blocks * a.splits_kv;
+    dq_part<T, DP, VEC>(a, smem, i % q_blocks, i / q_blocks);
+  }
+}
+
+// Sums the shares' partial rows in their order, a wave per row: blockIdx.y 0 dQ
+// from part_q [splits_q][rows][DP], 1 and 2 dK and dV from part_kv
+// [splits_kv][2][rows][DP]; `from` where the first is not wanted.
 template <typename T, int DP>
-__global__ __launch_bounds__(256) void xattn_sum_kernel(const float* __restrict__ part, XTensor first, XTensor second,
-                                                        int planes, int splits, int batch, int heads, int len, int d) {
+__global__ __launch_bounds__(256) void xattn_sum_kernel(XAttnArgs a, int from) {
   using E = typename Elem<T>::type;
   constexpr int PL = DP / 64;
   const int lane = threadIdx.x & 63;
-  const size_t rows = static_cast<size_t>(batch) * heads * len;
+  const int which = blockIdx.y + from;
+  const int heads = which == 0 ? a.heads : a.kv_heads;
+  const int len = which == 0 ? a.q_len : a.kv_len;
+  const size_t rows = static_cast<size_t>(a.batch) * heads * len;
   const size_t row = static_cast<size_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
   if (row >= rows) {
     return;
@@ -1096,20 +1133,22 @@ __global__ __launch_bounds__(256) void xattn_sum_kernel(const float* __restrict_
   const int problem = static_cast<int>(row / len);
   const int64_t pos = static_cast<int64_t>(row - static_cast<size_t>(problem) * len);
   const int b = problem / heads;
-  const XTensor x = blockIdx.y == 0 ? first : second;
+  const XTensor& x = which == 0 ? a.dq : which == 1 ? a.dk : a.dv;
+  const int splits = which == 0 ? a.splits_q : a.splits_kv;
+  const size_t step = (which == 0 ? 1 : 2) * rows * DP;
+  const float* p = (which == 0 ? a.part_q : a.part_kv) + ((which == 2 ? rows : 0) + row) * DP + lane;
   float s[PL] = {};
 #pragma unroll 8
   for (int z = 0; z < splits; ++z) {
-    const float* p = part + ((static_cast<size_t>(z) * planes + blockIdx.y) * rows + row) * DP + lane;
 #pragma unroll
     for (int i = 0; i < PL; ++i) {
-      s[i] += p[i * 64];
+      s[i] += p[z * step + i * 64];
     }
   }
   E* out = static_cast<E*>(x.p) + b * x.sb + (problem - b * heads) * x.sh + pos * x.ss;
 #pragma unroll
   for (int i = 0; i < PL; ++i) {
-    if (i * 64 + lane < d) {
+    if (i * 64 + lane < a.d) {
       out[i * 64 + lane] = from_f32<T>(s[i]);
     }
   }
@@ -1135,38 +1174,67 @@ hipError_t launch_lds(K kernel, hipError_t allowed, dim3 grid, size_t lds, const
                       static_cast<int>(lds))
 
 template <typename T, int DP, bool VEC>
-hipError_t launch(XAttnStep step, const XAttnArgs& a, hipStream_t stream) {
+hipError_t launch_forward(const XAttnArgs& a, hipStream_t stream) {
   const unsigned problems = static_cast<unsigned>(a.batch * a.kv_heads);
-  const int rows = a.heads / a.kv_heads * a.q_len;
+  const unsigned rows = static_cast<unsigned>(a.heads / a.kv_heads * a.q_len);
   const unsigned z = static_cast<unsigned>(a.splits);
   constexpr size_t lds = tiles_bytes<T, DP>();
-  const dim3 by_rows(problems, static_cast<unsigned>((rows + 127) / 128), z);
-  if (step == XAttnStep::kForward && a.few) {
+  if (a.few) {
     static const hipError_t allowed = LC_XATTN_ALLOW((xattn_few_kernel<T, DP, VEC>), 2 * lds);
-    return launch_lds(xattn_few_kernel<T, DP, VEC>, allowed,
-                      dim3(problems, static_cast<unsigned>((rows + 31) / 32), z), 2 * lds, a, stream);
+    return launch_lds(xattn_few_kernel<T, DP, VEC>, allowed, dim3(problems, (rows + 31) / 32, z), 2 * lds, a, stream);
   }
-  if (step == XAttnStep::kForward) {
-    static const hipError_t allowed = LC_XATTN_ALLOW((xattn_fwd_kernel<T, DP, VEC>), lds);
-    return launch_lds(xattn_fwd_kernel<T, DP, VEC>, allowed, by_rows, lds, a, stream);
+  static const hipError_t allowed = LC_XATTN_ALLOW((xattn_fwd_kernel<T, DP, VEC>), lds);
+  return launch_lds(xattn_fwd_kernel<T, DP, VEC>, allowed, dim3(problems, (rows + 127) / 128, z), lds, a, stream);
+}
+
+template <typename T, int DP, bool VEC>
+hipError_t launch_backward(const XAttnArgs& a, hipStream_t stream) {
+  const size_t rows_q = static_cast<size_t>(a.batch) * a.heads * a.q_len;
+  const size_t rows_kv = static_cast<size_t>(a.batch) * a.kv_heads * a.kv_len;
+  if (rows_q != 0) {
+    xattn_delta_kernel<T, VEC><<<static_cast<unsigned>((rows_q + 15) / 16), 256, 0, stream>>>(a);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) {
+      return e;
+    }
   }
-  if (step == XAttnStep::kGradQ) {
-    static const hipError_t allowed = LC_XATTN_ALLOW((xattn_dq_kernel<T, DP, VEC>), lds);
-    return launch_lds(xattn_dq_kernel<T, DP, VEC>, allowed, by_rows, lds, a, stream);
+  const unsigned group_rows = static_cast<unsigned>(a.heads / a.kv_heads * a.q_len);
+  const unsigned blocks = static_cast<unsigned>((a.kv_len + 127) / 128 * a.splits_kv) +
+                          (group_rows + 127) / 128 * static_cast<unsigned>(a.splits_q);
+  constexpr size_t tiles = tiles_bytes<T, DP>();
+  constexpr size_t own = dkv_lds_bytes<T, DP>();
+  constexpr size_t lds = tiles > own ? tiles : own;
+  if (blocks != 0) {
+    static const hipError_t allowed = LC_XATTN_ALLOW((xattn_bwd_kernel<T, DP, VEC>), lds);
+    const hipError_t e = launch_lds(xattn_bwd_kernel<T, DP, VEC>, allowed,
+                                    dim3(static_cast<unsigned>(a.batch * a.kv_heads), blocks), lds, a, stream);
+    if (e != hipSuccess) {
+      return e;
+    }
   }
-  constexpr size_t kv_lds = dkv_lds_bytes<T, DP>();
-  static const hipError_t allowed = LC_XATTN_ALLOW((xattn_dkv_kernel<T, DP, VEC>), kv_lds);
-  return launch_lds(xattn_dkv_kernel<T, DP, VEC>, allowed,
-                    dim3(problems, static_cast<unsigned>((a.kv_len + 127) / 128), z), kv_lds, a, stream);
+  const bool sum_q = a.splits_q > 1;
+  const bool sum_kv = a.splits_kv > 1;
+  if (sum_q || sum_kv) {
+    const size_t rows = sum_q && (!sum_kv || rows_q > rows_kv) ? rows_q : rows_kv;
+    const dim3 grid(static_cast<unsigned>((rows + 3) / 4), (sum_q ? 1 : 0) + (sum_kv ? 2 : 0));
+    xattn_sum_kernel<T, DP><<<grid, 256, 0, stream>>>(a, sum_q ? 0 : 1);
+  }
+  return hipGetLastError();
 }
 #undef LC_XATTN_ALLOW
 
 template <typename T>
-hipError_t launch_type(XAttnStep step, const XAttnArgs& a, bool vec, hipStream_t stream) {
+hipError_t launch_type(bool backward, const XAttnArgs& a, bool vec, hipStream_t stream) {
   if (a.d <= 64) {
-    return vec ? launch<T, 64, true>(step, a, stream) : launch<T, 64, false>(step, a, stream);
+    if (backward) {
+      return vec ? launch_backward<T, 64, true>(a, stream) : launch_backward<T, 64, false>(a, stream);
+    }
+    return vec ? launch_forward<T, 64, true>(a, stream) : launch_forward<T, 64, false>(a, stream);
   }
-  return vec ? launch<T, 128, true>(step, a, stream) : launch<T, 128, false>(step, a, stream);
+  if (backward) {
+    return vec ? launch_backward<T, 128, true>(a, stream) : launch_backward<T, 128, false>(a, stream);
+  }
+  return vec ? launch_forward<T, 128, true>(a, stream) : launch_forward<T, 128, false>(a, stream);
 }
 
 template <typename T>
@@ -1181,35 +1249,30 @@ hipError_t join_type(const XAttnArgs& a, hipStream_t stream) {
   return hipGetLastError();
 }
 
-template <typename T>
-hipError_t sum_type(const float* part, const XTensor& x, const XTensor* second, int splits, int batch, int heads,
-                    int len, int d, hipStream_t stream) {
-  const size_t rows = static_cast<size_t>(batch) * heads * len;
-  const int planes = second != nullptr ? 2 : 1;
-  const dim3 grid(static_cast<unsigned>((rows + 3) / 4), planes);
-  const XTensor& y = second != nullptr ? *second : x;
-  if (d <= 64) {
-    xattn_sum_kernel<T, 64><<<grid, 256, 0, stream>>>(part, x, y, planes, splits, batch, heads, len, d);
-  } else {
-    xattn_sum_kernel<T, 128><<<grid, 256, 0, stream>>>(part, x, y, planes, splits, batch, heads, len, d);
-  }
-  return hipGetLastError();
-}
-
 }  // namespace
 }  // namespace lchip::k
 
 namespace lchip::kern {
 
-hipError_t crossAttention(XAttnStep step, const XAttnArgs& a, DType type, bool aligned, hipStream_t stream) {
+namespace {
+hipError_t launch(bool backward, const XAttnArgs& a, DType type, bool aligned, hipStream_t stream) {
   switch (type) {
     case DType::kF32:
-      return k::launch_type<k::F32>(step, a, aligned, stream);
+      return k::launch_type<k::F32>(backward, a, aligned, stream);
     case DType::kBF16:
-      return k::launch_type<k::BF16>(step, a, aligned, stream);
+      return k::launch_type<k::BF16>(backward, a, aligned, stream);
     default:
-      return k::launch_type<k::F16>(step, a, aligned, stream);
+      return k::launch_type<k::F16>(backward, a, aligned, stream);
   }
+}
+}  // namespace
+
+hipError_t crossAttentionForward(const XAttnArgs& a, DType type, bool aligned, hipStream_t stream) {
+  return launch(false, a, type, aligned, stream);
+}
+
+hipError_t crossAttentionBackward(const XAttnArgs& a, DType type, bool aligned, hipStream_t stream) {
+  return launch(true, a, type, aligned, stream);
 }
 
 hipError_t crossAttentionJoin(const XAttnArgs& a, DType type, hipStream_t stream) {
@@ -1220,18 +1283,6 @@ hipError_t crossAttentionJoin(const XAttnArgs& a, DType type, hipStream_t stream
       return k::join_type<k::BF16>(a, stream);
     default:
       return k::join_type<k::F16>(a, stream);
-  }
-}
-
-hipError_t crossAttentionSum(const float* part, const XTensor& x, const XTensor* second, int splits, int batch,
-                             int heads, int len, int d, DType type, hipStream_t stream) {
-  switch (type) {
-    case DType::kF32:
-      return k::sum_type<k::F32>(part, x, second, splits, batch, heads, len, d, stream);
-    case DType::kBF16:
-      return k::sum_type<k::BF16>(part, x, second, splits, batch, heads, len, d, stream);
-    default:
-      return k::sum_type<k::F16>(part, x, second, splits, batch, heads, len, d, stream);
   }
 }
 

@@ -10,8 +10,8 @@ namespace {
 
 constexpr const char* kOp = "kv cache";
 constexpr std::size_t kMost = std::size_t{1} << 30;
-// Workgroups of four waves that fill the chip.
-constexpr std::size_t kTarget = 512;
+// Workgroups of four waves that run at once.
+constexpr std::size_t kSlots = 512;
 constexpr std::size_t kRows = 16;  // query rows of a workgroup
 
 Status checkCache(const lcKvCache* c) {
@@ -146,7 +146,7 @@ Status checkAttn(const lcKvCache* cache, const lcKvAttentionConfig* cfg, AttnPla
   plan->width = static_cast<std::size_t>(kern::kXAttnWidth(static_cast<int>(cache->head_dim)));
   const std::size_t blocks = cfg->batch * cache->kv_heads * ((group * cfg->q_len + kRows - 1) / kRows);
   // A split has at least a page for each of its four waves.
-  plan->splits = splitCount(blocks, (cfg->table_width + 3) / 4, kTarget);
+  plan->splits = splitCount(blocks, (cfg->table_width + 3) / 4, kSlots, 1.0, 3.0);
   return Status::kSuccess;
 }
 
