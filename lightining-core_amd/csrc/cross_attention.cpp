@@ -26,7 +26,8 @@ constexpr double kJoin = 3.0;
 // result cost more than its work.
 constexpr double kShare = 0.8;
 constexpr std::size_t kMostShares = 32;
-constexpr double kLeast = 8.0;
+constexpr double kLeast = 40.0;     // 16-bit types
+constexpr double kLeastF32 = 12.0;  // fp32 products take eight times as long
 
 // How the kernels share the work of a problem, and the workspace that it
 // takes: a function of the shape alone, so that the size a caller asks for is
@@ -69,7 +70,7 @@ Plan planOf(const lcCrossAttentionConfig& c) {
   const double work_q = 3.0 * static_cast<double>(tile / 32 * kv_tiles);  // of one block
   const double work_kv = 4.0 * static_cast<double>(q_tiles);
   const double all = work_q * static_cast<double>(q_blocks) + work_kv * static_cast<double>(kv_blocks);
-  const double most = std::max(kLeast, kShare * all / static_cast<double>(kSlots));
+  const double most = std::max(c.dtype == LC_DTYPE_F32 ? kLeastF32 : kLeast, kShare * all / static_cast<double>(kSlots));
   const auto shares = [most](double work, std::size_t tiles) {
     const std::size_t want = static_cast<std::size_t>(std::ceil(work / most));
     return static_cast<int>(std::max<std::size_t>(1, std::min({want, tiles, kMostShares})));

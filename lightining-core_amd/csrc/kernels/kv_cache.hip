@@ -65,8 +65,8 @@ __global__ __launch_bounds__(256) void kv_store_kernel(KvStoreArgs a) {
   using E = typename Elem<T>::type;
   __shared__ float tops[2][4];
   const int b = blockIdx.z;
-  const int h = blockIdx.y;
-  const int p = blockIdx.x;
+  const int h = blockIdx.x;
+  const int p = blockIdx.y;
   const int len = min(max(a.lengths == nullptr ? a.kv_len : a.lengths[b], 0), a.kv_len);
   const int left = min(len - p * kPage, kPage);
   if (left <= 0) {
@@ -479,7 +479,9 @@ __global__ __launch_bounds__(256, 2) void kv_attn_kernel(KvAttnArgs a) {
 
 template <typename T>
 hipError_t store_type(const KvStoreArgs& a, bool aligned, hipStream_t stream) {
-  const dim3 grid(static_cast<unsigned>((a.kv_len + kPage - 1) / kPage), static_cast<unsigned>(a.heads),
+  // Heads first: of tokens whose rows hold all heads, workgroups that run at once
+  // then read neighbouring parts.
+  const dim3 grid(static_cast<unsigned>(a.heads), static_cast<unsigned>((a.kv_len + kPage - 1) / kPage),
                   static_cast<unsigned>(a.batch));
   if (aligned) {
     kv_store_kernel<T, true><<<grid, 256, 0, stream>>>(a);

@@ -75,7 +75,7 @@ Status store(const lcKvCache* cache, std::size_t batch, std::size_t kv_len, lcDa
   if (!validDtype(dtype)) {
     return fail(Status::kInvalidValue, "kv cache: dtype must be f32, bf16 or f16");
   }
-  if (batch > 65535 || kv_len > kMost) {
+  if (batch > 65535 || kv_len > std::size_t{65535} * kern::kKvPage) {
     return fail(Status::kNotSupported, "kv cache: shape too large");
   }
   kern::KvStoreArgs a{};
