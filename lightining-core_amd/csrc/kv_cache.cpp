@@ -145,8 +145,13 @@ Status checkAttn(const lcKvCache* cache, const lcKvAttentionConfig* cfg, AttnPla
   plan->rows = cfg->batch * cfg->heads * cfg->q_len;
   plan->width = static_cast<std::size_t>(kern::kXAttnWidth(static_cast<int>(cache->head_dim)));
   const std::size_t blocks = cfg->batch * cache->kv_heads * ((group * cfg->q_len + kRows - 1) / kRows);
-  // A split has at least a page for each of its four waves.
-  plan->splits = splitCount(blocks, (cfg->table_width + 3) / 4, kSlots, 1.0, 3.0);
+  // A split has at least a page for each of its four waves.  Rows differ in
+  // length and the host does not know by how much: long tables are split twice as
+  // often as would fill the chip, so that short rows' workgroups make room (32
+  // rows of 64 to 128 pages: 85.5 -> 80.9 us; four times as often 85.0).
+  const std::size_t quads = (cfg->table_width + 3) / 4;
+  const int splits = splitCount(blocks, quads, kSlots, 1.0, 3.0);
+  plan->splits = quads >= 8u * splits ? 2 * splits : splits;
   return Status::kSuccess;
 }
 
