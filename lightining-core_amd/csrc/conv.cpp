@@ -348,6 +348,7 @@ Status vitForwardDevice(HipContext* ctx, lcVitBlockSession* s) {
     ln.n = E;
     ln.sx = ln.sy = E;
     ln.wide = 1;
+    ln.weights_aligned = c.embed % 4 == 0 ? 1 : 0;  // the bias lies behind the weight
     ln.eps = s->norm_eps;
     e = kern::layerNorm(ln, c.compute_dtype == LC_DTYPE_F16 ? kern::DType::kF16 : kern::DType::kBF16, false, true,
                         ctx->stream);

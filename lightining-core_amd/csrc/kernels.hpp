@@ -400,6 +400,7 @@ struct LayerNormArgs {
   int64_t sx, sy, sdx;
   int n;
   int wide;  // w, b, dw and db are fp32 (else x's type)
+  int weights_aligned;  // w and b lie on 16 bytes
   float eps;
 };
 // chunk: values of x in 16 bytes.

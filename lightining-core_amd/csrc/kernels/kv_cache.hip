@@ -399,24 +399,22 @@ __global__ __launch_bounds__(256, 2) void kv_attn_kernel(KvAttnArgs a) {
       }
       terms<NP>(v, pt[u]);
     }
-    if (left < kPage) {
-      // Codes behind the last token may be anything: a NaN there must not meet
-      // its probability of zero.
+    // Codes behind the last token may be anything: a NaN there must not meet its
+    // probability of zero.  (Every page is masked, 4 instructions a load: with a
+    // branch around it the compiler gave registers of V to the probabilities'
+    // terms while V was still needed.)
+    u32x4 keep;
 #pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        const int keep = min(max(left - 16 * g - 4 * w, 0), 4);
-        const uint32_t mask = keep == 4 ? 0xffffffffu : (1u << (8 * keep)) - 1u;
-#pragma unroll
-        for (int t = 0; t < DW / 16; ++t) {
-          vr[t][w] &= mask;
-        }
-      }
+    for (int w = 0; w < 4; ++w) {
+      const int n = min(max(left - 16 * g - 4 * w, 0), 4);
+      keep[w] = n == 4 ? 0xffffffffu : (1u << (8 * n)) - 1u;
     }
 #pragma unroll
     for (int t = 0; t < DW / 16; ++t) {
+      const u32x4 v = vr[t] & keep;
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        const u32x4 vw = widen(vr[t][2 * u], vr[t][2 * u + 1]);
+        const u32x4 vw = widen(v[2 * u], v[2 * u + 1]);
 #pragma unroll
         for (int n = 0; n < NP; ++n) {
           o[t] = mfma16x16x32<BF16>(vw, pt[u][n], o[t]);

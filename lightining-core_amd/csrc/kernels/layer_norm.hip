@@ -51,6 +51,46 @@ template <typename T>
 __device__ __forceinline__ float weight_at(const void* w, int wide, int i) {
   return wide ? static_cast<const float*>(w)[i] : to_f32<T>(static_cast<const typename Elem<T>::type*>(w)[i]);
 }
+// Chunk `chunk` of the weights (as many as x's chunk holds), `none` where there
+// are none; zeros past their end.
+template <typename T, bool VEC>
+__device__ __forceinline__ void load_weights(const void* w, const LayerNormArgs& a, int chunk, float none,
+                                             float (&v)[Elem<T>::kChunk]) {
+  constexpr int EC = Elem<T>::kChunk;
+  const int at = chunk * EC;
+#pragma unroll
+  for (int i = 0; i < EC; ++i) {
+    v[i] = at + i < a.n ? none : 0.0f;
+  }
+  if (w == nullptr || at >= a.n) {
+    return;
+  }
+  if (VEC && a.weights_aligned) {
+    if (a.wide) {
+#pragma unroll
+      for (int j = 0; j < EC / 4; ++j) {
+        const float4 f = *reinterpret_cast<const float4*>(static_cast<const float*>(w) + at + 4 * j);
+        v[4 * j] = f.x;
+        v[4 * j + 1] = f.y;
+        v[4 * j + 2] = f.z;
+        v[4 * j + 3] = f.w;
+      }
+    } else {
+      const u32x4 c = *reinterpret_cast<const u32x4*>(static_cast<const typename Elem<T>::type*>(w) + at);
+#pragma unroll
+      for (int i = 0; i < EC; ++i) {
+        v[i] = chunk_value<T>(c, i);
+      }
+    }
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < EC; ++i) {
+    if (at + i < a.n) {
+      v[i] = weight_at<T>(w, a.wide, at + i);
+    }
+  }
+}
 template <typename T>
 __device__ __forceinline__ void put_weight(void* w, int wide, int i, float v) {
   if (wide) {
@@ -98,15 +138,6 @@ __global__ __launch_bounds__(kThreads) void ln_fwd_kernel(LayerNormArgs a) {
   const int lane = threadIdx.x % LANES;
   const int64_t step = static_cast<int64_t>(gridDim.x) * RPB;
   float w[CH][EC], bias[CH][EC];
-#pragma unroll
-  for (int c = 0; c < CH; ++c) {
-#pragma unroll
-    for (int i = 0; i < EC; ++i) {
-      const int at = (c * LANES + lane) * EC + i;
-      w[c][i] = a.w != nullptr && at < a.n ? weight_at<T>(a.w, a.wide, at) : 1.0f;
-      bias[c][i] = a.b != nullptr && at < a.n ? weight_at<T>(a.b, a.wide, at) : 0.0f;
-    }
-  }
   const float n = static_cast<float>(a.n);
   int flip = 0;
   // All threads of a workgroup make the same number of rounds (barriers).
@@ -122,6 +153,11 @@ __global__ __launch_bounds__(kThreads) void ln_fwd_kernel(LayerNormArgs a) {
     }
   };
   fetch(row);
+#pragma unroll
+  for (int c = 0; c < CH; ++c) {
+    load_weights<T, VEC>(a.w, a, c * LANES + lane, 1.0f, w[c]);
+    load_weights<T, VEC>(a.b, a, c * LANES + lane, 0.0f, bias[c]);
+  }
   for (int64_t k = 0; k < rounds; ++k, row += step) {
     float x[CH][EC];
     float s = 0.0f;
@@ -234,8 +270,6 @@ __global__ __launch_bounds__(kThreads) void ln_bwd_kernel(LayerNormArgs a) {
   for (int c = 0; c < CH; ++c) {
 #pragma unroll
     for (int i = 0; i < EC; ++i) {
-      const int at = (c * LANES + lane) * EC + i;
-      w[c][i] = at < a.n ? (a.w != nullptr ? weight_at<T>(a.w, a.wide, at) : 1.0f) : 0.0f;
       dw[c][i] = 0.0f;
       db[c][i] = 0.0f;
     }
@@ -259,6 +293,10 @@ __global__ __launch_bounds__(kThreads) void ln_bwd_kernel(LayerNormArgs a) {
     rstd = a.rstd[at];
   };
   fetch(row);
+#pragma unroll
+  for (int c = 0; c < CH; ++c) {
+    load_weights<T, VEC>(a.w, a, c * LANES + lane, 1.0f, w[c]);
+  }
   for (int64_t k = 0; k < rounds; ++k, row += step) {
     const bool in = row < a.rows;
     const float mu = mean;

@@ -67,6 +67,8 @@ Status takeRows(const lcLayerNormConfig& c, const char* name, const void* p, std
   return Status::kSuccess;
 }
 
+bool onChunk(const void* p) { return reinterpret_cast<std::uintptr_t>(p) % 16 == 0; }
+
 Status checkWeight(const lcLayerNormConfig& c, const char* name, const void* p) {
   if (reinterpret_cast<std::uintptr_t>(p) % bytesOf(c.weight_dtype) != 0) {
     return fail(Status::kInvalidValue, std::string(kOp) + ": " + name + " is not aligned to its elements");
@@ -111,6 +113,7 @@ Status forward(const lcLayerNormConfig* cfg, const void* x, std::int64_t x_strid
   a.y = y;
   a.w = weight;
   a.b = bias;
+  a.weights_aligned = onChunk(weight) && onChunk(bias) ? 1 : 0;
   a.mean = mean;
   a.rstd = rstd;
   LC_HIP_TRY(kern::layerNorm(a, dtypeOf(c.dtype), false, aligned, static_cast<hipStream_t>(stream)));
@@ -157,6 +160,7 @@ Status backward(const lcLayerNormConfig* cfg, const void* dy, std::int64_t dy_st
   a.x = x;
   a.dy = dy;
   a.w = weight;
+  a.weights_aligned = onChunk(weight) ? 1 : 0;
   a.mean = const_cast<float*>(mean);
   a.rstd = const_cast<float*>(rstd);
   a.dx = dx;

@@ -168,6 +168,8 @@ ATTENTIONS = [
     (8, 8, 3, 48, [63, 300], 9),
     (16, 2, 5, 80, [130, 7], 0),      # rows of a head block cross 16
     (2, 2, 40, 112, [90], 0),
+    (16, 2, 5, 64, [200, 7], 0),      # blocks of rows that share whole pages' width
+    (8, 1, 3, 128, [130, 64, 0], 0),
     (32, 4, 1, 128, [4000, 1], 0),    # splits, and rows without their share
     (1, 1, 1, 32, [6400], 200),
 ]
