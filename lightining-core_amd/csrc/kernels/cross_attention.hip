@@ -811,8 +811,9 @@ __global__ __launch_bounds__(256) void xattn_delta_kernel(XAttnArgs a) {
 }
 
 // dQ of 128 rows (block `blk`) over share z of the keys: as the forward, with
-// dO's rows beside Q's.
-template <typename T, int DP, bool VEC>
+// dO's rows beside Q's.  DELTA: the rows' delta = sum over the keys of P dP
+// instead (of all keys, splits_q being ignored), with the exponent of dO.
+template <typename T, int DP, bool VEC, bool DELTA>
 __device__ __forceinline__ void dq_part(const XAttnArgs& a, char* smem, int blk, int z) {
   using TL = Tile<T, DP>;
   using E = typename Elem<T>::type;
@@ -832,7 +833,7 @@ __device__ __forceinline__ void dq_part(const XAttnArgs& a, char* smem, int blk,
   const QueryRow qr = query_row(valid ? r : 0, a.q_len, hk * group);
   const int len = keys_of(a, b);
   int t0, t1;
-  tile_range((len + KT - 1) / KT, a.splits_q, z, &t0, &t1);
+  tile_range((len + KT - 1) / KT, DELTA ? 1 : a.splits_q, z, &t0, &t1);
 
   Stream<T, DP, KT, VEC, 4> ks, vs;
   ks.init(static_cast<const E*>(a.k.p) + b * a.k.sb + hk * a.k.sh, a.k.ss, len, a.d, wave, lane);
@@ -855,13 +856,17 @@ __device__ __forceinline__ void dq_part(const XAttnArgs& a, char* smem, int blk,
   }
   const size_t lrow = (static_cast<size_t>(b) * a.heads + qr.head) * a.q_len + qr.pos;
   const float lse2 = valid ? a.lse[lrow] * kLog2e : 0.0f;
-  const float2 de = valid ? *reinterpret_cast<const float2*>(a.delta + 2 * lrow) : make_float2(0.0f, 0.0f);
+  float2 de = make_float2(0.0f, 0.0f);
+  if (!DELTA && valid) {
+    de = *reinterpret_cast<const float2*>(a.delta + 2 * lrow);
+  }
   const float delta = de.x;
   const int ex = static_cast<int>(de.y);
   float down = 1.0f;
-  if constexpr (__is_same(T, F16)) {
+  if constexpr (__is_same(T, F16) && !DELTA) {
     down = power_of_two(-ex);
   }
+  float sum = 0.0f;
   floatx16 dq[TL::DT];
 #pragma unroll
   for (int t = 0; t < TL::DT; ++t) {
@@ -893,7 +898,7 @@ __device__ __forceinline__ void dq_part(const XAttnArgs& a, char* smem, int blk,
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         const float p = fast_exp2(fmaf(s[i], c, -lse2));
-        s[i] = p * (dp[i] - delta) * down;
+        s[i] = DELTA ? p * dp[i] : p * (dp[i] - delta) * down;
       }
       if (tail) {
 #pragma unroll
@@ -903,7 +908,12 @@ __device__ __forceinline__ void dq_part(const XAttnArgs& a, char* smem, int blk,
           }
         }
       }
-      if constexpr (TL::EC == 8) {
+      if constexpr (DELTA) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          sum += s[i];
+        }
+      } else if constexpr (TL::EC == 8) {
         u32x4 pk[2];
         pack_block<T>(s, pk);
         __builtin_amdgcn_s_setprio(1);
@@ -914,6 +924,22 @@ __device__ __forceinline__ void dq_part(const XAttnArgs& a, char* smem, int blk,
       }
     }
     arrive();
+  }
+  if constexpr (DELTA) {
+    float amax = 0.0f;
+#pragma unroll
+    for (int x = 0; x < TL::NS; ++x) {
+#pragma unroll
+      for (int i = 0; i < TL::EC; ++i) {
+        amax = fmaxf(amax, fabsf(chunk_value<T>(gf[x], i)));
+      }
+    }
+    sum = add_xor32(sum);
+    amax = max_xor32(amax);
+    if (valid && half == 0) {
+      *reinterpret_cast<float2*>(a.delta + 2 * lrow) = make_float2(sum, static_cast<float>(exponent_of(amax)));
+    }
+    return;
   }
   if (!valid) {
     return;
@@ -1082,11 +1108,11 @@ __device__ __forceinline__ void dkv_part(const XAttnArgs& a, char* smem, int blk
     if constexpr (TL::EC == 8) {
       u32x4 pk[2];
       pack_block<T>(s, pk);
-      u32x4 pd[2];
-      pack_block<T>(dp, pd);
       // As in the forward: 383 -> 375 us for the whole pass at 2048 x 1500.
       __builtin_amdgcn_s_setprio(1);
       TL::transposed(gl, 0, pk, lane, dv);
+      u32x4 pd[2];
+      pack_block<T>(dp, pd);
       TL::transposed(ql, 0, pd, lane, dk);
       __builtin_amdgcn_s_setprio(0);
     } else {
@@ -1139,8 +1165,18 @@ __global__ __launch_bounds__(256, (VEC && (Elem<T>::kChunk == 8 || DP == 64) ? 2
   } else {
     const int q_blocks = (a.heads / a.kv_heads * a.q_len + 127) / 128;
     const int i = y - kv_blocks * a.splits_kv;
-    dq_part<T, DP, VEC>(a, smem, i % q_blocks, i / q_blocks);
+    dq_part<T, DP, VEC, false>(a, smem, i % q_blocks, i / q_blocks);
   }
+}
+
+// delta from the probabilities instead of from `out`: grid (problems, row
+// blocks).  A 16-bit `out` has lost 2^-9 of itself, and with few keys it is of
+// the values' own size: dQ and dK of 18 keys were 1.7 times as far from 64 bits
+// as a rounding of the exact ones is.  Two more products, for short keys only.
+template <typename T, int DP, bool VEC>
+__global__ __launch_bounds__(256, (waves_per_simd<T, DP, VEC>())) void xattn_delta_keys_kernel(XAttnArgs a) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  dq_part<T, DP, VEC, true>(a, smem, blockIdx.y, 0);
 }
 
 // Sums the shares' partial rows in their order, a wave per row: blockIdx.y 0 dQ
@@ -1220,16 +1256,25 @@ template <typename T, int DP, bool VEC>
 hipError_t launch_backward(const XAttnArgs& a, hipStream_t stream) {
   const size_t rows_q = static_cast<size_t>(a.batch) * a.heads * a.q_len;
   const size_t rows_kv = static_cast<size_t>(a.batch) * a.kv_heads * a.kv_len;
-  if (rows_q != 0) {
+  const unsigned q_blocks = static_cast<unsigned>((a.heads / a.kv_heads * a.q_len + 127) / 128);
+  constexpr bool k16 = Elem<T>::kChunk == 8;
+  if (k16 && rows_q != 0 && a.kv_len <= kern::kXAttnShortKeys) {
+    constexpr size_t lds = tiles_bytes<T, DP>();
+    static const hipError_t allowed = LC_XATTN_ALLOW((xattn_delta_keys_kernel<T, DP, VEC>), lds);
+    const hipError_t e = launch_lds(xattn_delta_keys_kernel<T, DP, VEC>, allowed,
+                                    dim3(static_cast<unsigned>(a.batch * a.kv_heads), q_blocks), lds, a, stream);
+    if (e != hipSuccess) {
+      return e;
+    }
+  } else if (rows_q != 0) {
     xattn_delta_kernel<T, VEC><<<static_cast<unsigned>((rows_q + 15) / 16), 256, 0, stream>>>(a);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) {
       return e;
     }
   }
-  const unsigned group_rows = static_cast<unsigned>(a.heads / a.kv_heads * a.q_len);
   const unsigned blocks = static_cast<unsigned>((a.kv_len + 127) / 128 * a.splits_kv) +
-                          (group_rows + 127) / 128 * static_cast<unsigned>(a.splits_q);
+                          q_blocks * static_cast<unsigned>(a.splits_q);
   constexpr size_t tiles = tiles_bytes<T, DP>();
   constexpr size_t own = dkv_lds_bytes<T, DP>();
   constexpr size_t lds = tiles > own ? tiles : own;

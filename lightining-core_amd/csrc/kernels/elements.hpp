@@ -74,6 +74,9 @@ __device__ __forceinline__ u32x4 load_chunk(const typename Elem<T>::type* row, i
     if (at < d) {
       r = *reinterpret_cast<const u32x4*>(row + at);
     }
+  } else if (at + EC <= d) {
+    // One load all the same: the hardware takes any alignment of an element.
+    __builtin_memcpy(&r, __builtin_assume_aligned(row + at, sizeof(*row)), 16);
   } else {
 #pragma unroll
     for (int i = 0; i < EC; ++i) {

@@ -106,20 +106,22 @@ __device__ __forceinline__ void store_chunk(typename Elem<T>::type* row, int chu
                                             const float (&v)[Elem<T>::kChunk]) {
   constexpr int EC = Elem<T>::kChunk;
   const int at = chunk * EC;
-  if constexpr (VEC) {
-    if (at < n) {
-      u32x4 c;
+  if (at + EC <= n) {
+    u32x4 c;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if constexpr (EC == 4) {
-          c[i] = __builtin_bit_cast(uint32_t, v[i]);
-        } else {
-          c[i] = pack2<T>(v[2 * i], v[2 * i + 1]);
-        }
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (EC == 4) {
+        c[i] = __builtin_bit_cast(uint32_t, v[i]);
+      } else {
+        c[i] = pack2<T>(v[2 * i], v[2 * i + 1]);
       }
-      *reinterpret_cast<u32x4*>(row + at) = c;
     }
-  } else {
+    if constexpr (VEC) {
+      *reinterpret_cast<u32x4*>(row + at) = c;
+    } else {
+      __builtin_memcpy(__builtin_assume_aligned(row + at, sizeof(*row)), &c, 16);
+    }
+  } else if constexpr (!VEC) {
 #pragma unroll
     for (int i = 0; i < EC; ++i) {
       if (at + i < n) {
