@@ -13,9 +13,17 @@ constexpr std::size_t kMostRows = std::size_t{1} << 30;
 // Workgroups that run at once on 256 CUs: two a CU, of the few-row forward one.
 constexpr std::size_t kSlots = 512;
 constexpr std::size_t kFewSlots = 256;
-// Up to so many query rows of a problem, the forward's waves share the keys
-// instead of the rows.
-constexpr std::size_t kFewRows = 64;
+// The forward's waves share the keys of 32 rows, instead of taking 32 rows each,
+// up to so many 32-row blocks in all: the keys need no second launch to be
+// joined and each wave's chain of tiles is a quarter as long.  Beyond, reading a
+// tile for 32 rows instead of 128 costs more.  Wide 16-bit tiles fill a CU's LDS
+// with one such workgroup, the others with half.  us, rows per wave -> shared
+// keys: 16 heads of 300 x 1400 x 128 (160 blocks) 27.2 -> 17.7, 32 of 500 x 1000
+// x 128 (512) 30.4 -> 26.2, 32 of 700 x 1400 x 128 (704) 39.1 -> 47.2; 32 of 1000
+// x 1400 x 64 (1024) 37.8 -> 26.9, 32 of 1200 x 500 x 64 (1216) 15.6 -> 19.6; fp32
+// 32 of 700 x 1400 x 128 201 -> 167.
+constexpr std::size_t kFewBlocksWide = 512;
+constexpr std::size_t kFewBlocks = 1024;
 // A workgroup's start and end, and a join, in tiles' time (splitCount).
 constexpr double kFixed = 2.0;
 constexpr double kJoin = 3.0;
@@ -60,7 +68,8 @@ Plan planOf(const lcCrossAttentionConfig& c) {
   const std::size_t q_blocks = problems * ((group * c.q_len + block - 1) / block);
   const std::size_t kv_tiles = (c.kv_len + tile - 1) / tile;
   const std::size_t few_rows = kern::kXAttnFewRows;
-  p.few = group * c.q_len <= kFewRows;
+  const bool wide = c.dtype != LC_DTYPE_F32 && c.head_dim > 64;
+  p.few = problems * ((group * c.q_len + few_rows - 1) / few_rows) <= (wide ? kFewBlocksWide : kFewBlocks);
   p.splits_fwd = p.few ? splitCount(problems * ((group * c.q_len + few_rows - 1) / few_rows), (kv_tiles + 3) / 4,
                                     kFewSlots, kFixed, kJoin)
                        : splitCount(q_blocks, kv_tiles, kSlots, kFixed, kJoin);
