@@ -102,6 +102,28 @@ def test_against_64_bits(lc, shape, dtype):
 
 
 @pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("shape", [
+    (4, 8, 8, 1100, 200, 64, [200, 131, 64, 0]),  # 128-row blocks, keys split
+    (4, 8, 8, 1100, 70, 128, [70, 65, 64, 1]),
+    (16, 8, 8, 640, 40, 64, None),                # enough of them: no split
+    (2, 64, 4, 300, 130, 128, [130, 129]),        # rows of a head cross blocks
+    (4, 8, 8, 1100, 66, 33, None),                # rows that no vector load suits
+], ids=lambda s: "x".join(str(x) for x in s[:6]))
+def test_many_rows_against_64_bits(lc, shape, dtype):
+    b, hq, hkv, sq, sk, d, lens = shape
+    gen = _gen(sq + sk + d)
+    t = DTYPES[dtype]
+    q = _tensor(gen, b, hq, sq, d, t, "bshd")
+    k, v = (_tensor(gen, b, hkv, sk, d, t, x) for x in ("bhsd", "bshd"))
+    lengths = None if lens is None else torch.tensor(lens, dtype=torch.int32, device="cuda")
+    if lens is not None:
+        for i, n in enumerate(lens):
+            k[i, :, n:] = math.nan
+            v[i, :, n:] = math.nan
+    _check(lc, q, k, v, lengths, what=f"{shape} {dtype}")
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
 def test_bases_and_strides_off_alignment(lc, dtype):
     gen = _gen(7)
     t = DTYPES[dtype]
