@@ -488,7 +488,8 @@ lcError_t lcHipBackendStream(lcStream* out);
 lcError_t lcHipDeviceIndex(int* out);
 
 /* A [batch, heads, rows, d] tensor; d is contiguous, the strides count
- * elements and are not negative.  An input's may be zero (broadcast). */
+ * elements and are not negative.  An input's may be zero (broadcast).  A row
+ * stride whose 128 rows pass 2^31 bytes is LC_NOT_SUPPORTED. */
 typedef struct lcDeviceTensor {
   void* data;
   int64_t stride_batch;

@@ -65,7 +65,7 @@ Status takeTensor(const char* op, const char* name, const lcDeviceTensor* t, std
   }
   const std::int64_t most = std::int64_t{1} << 46;  // elements: no address product overflows
   if (out->sb > most || out->sh > most ||
-      out->ss > static_cast<std::int64_t>(((std::size_t{1} << 31) - 4096) / (64 * bytes))) {
+      out->ss > static_cast<std::int64_t>(((std::size_t{1} << 31) - 4096) / (128 * bytes))) {
     return fail(Status::kNotSupported, who + " has a stride too large");
   }
   if (written) {

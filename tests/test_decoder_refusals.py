@@ -61,7 +61,7 @@ def test_cross_attention_tensors():
     assert call(k=(256, 256, 256, -64)) == (N.LC_INVALID_VALUE, "cross attention: k has a negative stride")
     assert call(out=(256, 256, 128, 63))[0] == N.LC_INVALID_VALUE
     assert call(out=(256, 256, 0, 64))[0] == N.LC_INVALID_VALUE  # two heads written to one place
-    assert call(k=(256, 256, 256, 1 << 25))[0] == N.LC_NOT_SUPPORTED
+    assert call(k=(256, 256, 256, 1 << 23))[0] == N.LC_NOT_SUPPORTED  # 128 rows pass 2^31 bytes
     assert lib.lcCrossAttentionForward(ctypes.byref(cfg), None, None, None, None, None, None, None, 0,
                                        None) == N.LC_INVALID_VALUE
     assert lib.lcCrossAttentionBackward(ctypes.byref(cfg), *[None] * 5, None, None, None, None, None, None, 0,

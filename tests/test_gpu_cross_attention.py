@@ -258,11 +258,11 @@ def _plain(q, k, v, lengths):
 
 
 def test_offsets_past_32_bits(lc):
-    """Rows 16 M values apart: a head's keys span 9 GB."""
+    """Rows 8 M values apart, the widest that is taken: a head's keys span 9 GB."""
     if torch.cuda.mem_get_info()[0] < 40 << 30:
         pytest.skip("needs 40 GB of free memory")
     gen = _gen(15)
-    stride, sk = 16_000_000, 300
+    stride, sk = 8_000_000, 600
     mem = torch.empty(sk * stride, dtype=torch.bfloat16, device="cuda")
     k = mem.as_strided((1, 1, sk, 64), (0, 0, stride, 1))
     v = mem.as_strided((1, 1, sk, 64), (0, 0, stride, 1), 64)
@@ -276,6 +276,36 @@ def test_offsets_past_32_bits(lc):
     far = lc.cross_attention_backward(q, q, k.expand(1, 1, sk, 64), v, out, lse)
     near = lc.cross_attention_backward(q, q, kc, vc, out, lse)
     assert all(torch.equal(x, y) for x, y in zip(far, near))
+
+
+def test_a_capture_may_be_the_first_call():
+    """In a process of its own: the library's first call of all is captured."""
+    import os
+    import subprocess
+    import sys
+
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    code = """
+import sys
+sys.path.insert(0, %r)
+import torch
+q, k = (torch.randn(1, 2, s, 64, device="cuda") for s in (5, 700))
+x = torch.randn(9, 64, device="cuda")
+torch.cuda.synchronize()
+import lightning_core as lc
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    out = lc.cross_attention(q, k, k)
+    y = lc.layer_norm(x)
+for _ in range(3):
+    q.normal_(); x.normal_()
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, lc.cross_attention(q, k, k)) and torch.equal(y, lc.layer_norm(x))
+print("fine")
+""" % os.path.join(root, "lightining-core_amd")
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=100)
+    assert r.returncode == 0 and "fine" in r.stdout, r.stdout[-500:] + r.stderr[-1500:]
 
 
 @pytest.mark.parametrize("dtype", list(DTYPES))
