@@ -229,11 +229,18 @@ struct Stream {
   }
 };
 
+// This wave's LDS reads so far have returned (the empty asm keeps the compiler
+// from moving one behind the wait): what they read may be overwritten.
+__device__ __forceinline__ void reads_done() {
+  asm volatile("" ::: "memory");
+  wait_lgkmcnt<0>();
+}
+
 // Everything staged before has arrived, for every wave, and every wave is done
 // reading what it read before.
 __device__ __forceinline__ void arrive() {
+  reads_done();
   wait_vmcnt<0>();
-  wait_lgkmcnt<0>();
   stage_barrier();
 }
 
@@ -630,7 +637,7 @@ __global__ __launch_bounds__(256, 1) void xattn_few_kernel(XAttnArgs a) {
     asm volatile("" ::: "memory");
     floatx16 s[NB];
     w.scores(kl, s);
-    wait_lgkmcnt<0>();
+    reads_done();
     const bool more = t + 4 < t1;
     if (more) {
       ks.stage(t + 4, kl);
@@ -644,7 +651,7 @@ __global__ __launch_bounds__(256, 1) void xattn_few_kernel(XAttnArgs a) {
     }
     asm volatile("" ::: "memory");
     w.values(vl, s);
-    wait_lgkmcnt<0>();
+    reads_done();
     if (more) {
       vs.stage(t + 4, vl);
     }

@@ -172,11 +172,14 @@ ATTENTIONS = [
     (8, 1, 3, 128, [130, 64, 0], 0),
     (32, 4, 1, 128, [4000, 1], 0),    # splits, and rows without their share
     (1, 1, 1, 32, [6400], 200),
+    (2, 1, 1, 64, list(range(131)), 0),   # every length of a last page
+    (3, 1, 6, 128, list(range(131)), 0),
+    (2, 1, 1, 80, list(range(131)), 0),
 ]
 
 
 @pytest.mark.parametrize("dtype", list(DTYPES))
-@pytest.mark.parametrize("case", ATTENTIONS, ids=str)
+@pytest.mark.parametrize("case", ATTENTIONS, ids=lambda c: str(c)[:40])
 def test_attention(lc, case, dtype):
     hq, hkv, sq, d, lengths, width = case
     gen = _gen(hq + d + sum(lengths))
