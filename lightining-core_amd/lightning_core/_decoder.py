@@ -24,6 +24,11 @@ import numpy as np
 from . import _native as N
 from ._core import _check, _lib
 
+try:  # the compiled call helper, built next to the C library
+    from ._addr import invoke as _invoke
+except ImportError:  # not built: ctypes (slower, same result)
+    _invoke = None
+
 __all__ = ["cross_attention", "cross_attention_backward", "layer_norm", "layer_norm_backward", "kv_cache_store",
            "kv_cache_attention", "KV_PAGE_TOKENS"]
 
@@ -141,8 +146,36 @@ class _Torch:
     def finish(*results):
         return results
 
+    def run(self, name, spec, args, names):
+        """Calls the entry point (spec: csrc/pyaddr.c; names: its 't' arguments')."""
+        if _invoke is None:
+            return _run_ctypes(self, name, spec, args, names)
+        entry = _entries.get(name)
+        if entry is None:
+            entry = _entries[name] = ctypes.cast(getattr(_lib(), name), ctypes.c_void_p).value
+        status = _invoke(entry, spec, *args)
+        if status:
+            if status < 0:
+                raise ValueError(f"{names.split()[-1 - status]}'s last dimension must be contiguous")
+            _check(status)
+
 
 _torch_calls = {}
+_entries = {}  # entry point -> its address
+
+
+def _run_ctypes(call, name, spec, args, names):
+    """The same call through ctypes."""
+    names = iter(names.split())
+    got = []
+    for kind, x in zip(spec, args):
+        if kind == "t":
+            got.append(_tensor4(call, x, next(names)))
+        elif kind == "p":
+            got.append(None if x is None else call.addr(x))
+        else:
+            got.append(x)
+    _check(getattr(_lib(), name)(*got))
 
 
 def _torch_call(x):
@@ -241,6 +274,9 @@ class _Numpy:
         n = x.shape[-1]
         return (x.size // n if n else 0), n
 
+    def run(self, name, spec, args, names):
+        _run_ctypes(self, name, spec, args, names)
+
     def finish(self, *results):
         _check(_lib().lcDeviceSynchronize())
         for x in results:
@@ -254,16 +290,21 @@ def _call_of(first):
     return _torch_call(first) if _is_torch(first) else _Numpy()
 
 
+class _Struct:
+    """A ctypes structure and its address, which lives as long as this does."""
+
+    __slots__ = ("kept", "at")
+
+    def __init__(self, kept):
+        self.kept, self.at = kept, ctypes.addressof(kept)
+
+
 def _tensor4(call, x, name):
     """The library's view of a [batch, heads, rows, d] tensor."""
     st = call.strides(x)
     if st[3] != 1 and x.shape[3] > 1:
         raise ValueError(f"{name}'s last dimension must be contiguous")
     return _byref(N.DeviceTensor(call.addr(x), st[0], st[1], st[2]))
-
-
-def _addr(call, x):
-    return None if x is None else call.addr(x)
 
 
 def _same(x, shape, name):
@@ -327,7 +368,7 @@ def _xattn_plan(q_shape, k_shape, dtype, scale):
         n = ctypes.c_size_t()
         _check(_lib().lcCrossAttentionWorkspaceSize(_byref(cfg), backward, _byref(n)))
         got.append(n.value)
-    return _byref(cfg), got[0], got[1]
+    return _Struct(cfg), got[0], got[1]
 
 
 def _xattn_inputs(call, q, k, v, scale):
@@ -357,9 +398,8 @@ def cross_attention(q, k, v, kv_lengths=None, *, scale=None, return_lse=False, o
     out = _out(call, out, q, "out")
     lse = call.empty(q, q.shape[:3], N.LC_DTYPE_F32) if return_lse else None
     ws = call.workspace(nbytes)
-    _check(_lib().lcCrossAttentionForward(
-        cfg, _tensor4(call, q, "q"), _tensor4(call, k, "k"), _tensor4(call, v, "v"), _addr(call, lengths),
-        _tensor4(call, out, "out"), _addr(call, lse), _addr(call, ws), nbytes, call.stream))
+    call.run("lcCrossAttentionForward", "itttptppii", (cfg.at, q, k, v, lengths, out, lse, ws, nbytes, call.stream),
+             "q k v out")
     got = call.finish(out, lse)
     return got if return_lse else got[0]
 
@@ -383,10 +423,9 @@ def cross_attention_backward(dout, q, k, v, out, lse, kv_lengths=None, *, scale=
     lengths = _lengths(call, kv_lengths, q.shape[0])
     dq, dk, dv = call.empty_like(q), call.empty_like(k), call.empty_like(v)
     ws = call.workspace(nbytes)
-    _check(_lib().lcCrossAttentionBackward(
-        cfg, _tensor4(call, dout, "dout"), _tensor4(call, q, "q"), _tensor4(call, k, "k"), _tensor4(call, v, "v"),
-        _tensor4(call, out, "out"), call.addr(lse), _addr(call, lengths), _tensor4(call, dq, "dq"),
-        _tensor4(call, dk, "dk"), _tensor4(call, dv, "dv"), _addr(call, ws), nbytes, call.stream))
+    call.run("lcCrossAttentionBackward", "itttttpptttpii",
+             (cfg.at, dout, q, k, v, out, lse, lengths, dq, dk, dv, ws, nbytes, call.stream),
+             "dout q k v out dq dk dv")
     return call.finish(dq, dk, dv)
 
 
@@ -395,7 +434,7 @@ def _ln_plan(*key):
     cfg = N.LayerNormConfig(*key, 1)
     n = ctypes.c_size_t()
     _check(_lib().lcLayerNormWorkspaceSize(_byref(cfg), _byref(n)))
-    return _byref(cfg), n.value
+    return _Struct(cfg), n.value
 
 
 def _vector(call, x, n, dtype, name):
@@ -443,9 +482,8 @@ def layer_norm(x, weight=None, bias=None, *, eps=1e-5, return_stats=False):
     mean = rstd = None
     if return_stats:
         mean, rstd = call.empty(x, x.shape[:-1], N.LC_DTYPE_F32), call.empty(x, x.shape[:-1], N.LC_DTYPE_F32)
-    _check(_lib().lcLayerNormForward(
-        cfg, call.addr(x), stride, _addr(call, weight), _addr(call, bias), call.addr(y), n, _addr(call, mean),
-        _addr(call, rstd), call.stream))
+    call.run("lcLayerNormForward", "ipipppippi",
+             (cfg.at, x, stride, weight, bias, y, n, mean, rstd, call.stream), "")
     got = call.finish(y, mean, rstd)
     return got if return_stats else got[0]
 
@@ -477,9 +515,8 @@ def layer_norm_backward(dy, x, weight, mean, rstd):
     if weight is not None:
         dw, db = call.empty_contiguous(weight), call.empty_contiguous(weight)
     ws = call.workspace(nbytes)
-    _check(_lib().lcLayerNormBackward(
-        cfg, call.addr(dy), dy_stride, call.addr(x), stride, _addr(call, weight), call.addr(mean), call.addr(rstd),
-        call.addr(dx), n, _addr(call, dw), _addr(call, db), _addr(call, ws), nbytes, call.stream))
+    call.run("lcLayerNormBackward", "ipipippppipppii",
+             (cfg.at, dy, dy_stride, x, stride, weight, mean, rstd, dx, n, dw, db, ws, nbytes, call.stream), "")
     return call.finish(dx, dw, db)
 
 
@@ -531,9 +568,8 @@ def kv_cache_store(k, v, block_table, kv_lengths, k_pages, v_pages, k_scales, v_
         raise ValueError("k and the cache must agree in kv_heads and head_dim")
     lengths = _lengths(call, kv_lengths, b)
     t, stride = _table(call, block_table, b)
-    _check(_lib().lcKvCacheStore(
-        _byref(c), b, sk, call.dtype(k, "k"), _tensor4(call, k, "k"), _tensor4(call, v, "v"), call.addr(t), t.shape[1],
-        stride, _addr(call, lengths), call.stream))
+    call.run("lcKvCacheStore", "iiiittpiipi",
+             (ctypes.addressof(c), b, sk, call.dtype(k, "k"), k, v, t, t.shape[1], stride, lengths, call.stream), "k v")
     call.finish(*pool)
 
 
@@ -544,7 +580,7 @@ def _kv_plan(pages, kv_heads, d, b, hq, sq, width, dtype, scale):
     cfg = N.KvAttentionConfig(b, hq, sq, width, dtype, scale)
     n = ctypes.c_size_t()
     _check(_lib().lcKvCacheAttentionWorkspaceSize(_byref(cache), _byref(cfg), _byref(n)))
-    return _byref(cfg), n.value
+    return _Struct(cfg), n.value
 
 
 def kv_cache_attention(q, k_pages, v_pages, k_scales, v_scales, block_table, kv_lengths=None, *, scale=None,
@@ -572,8 +608,7 @@ def kv_cache_attention(q, k_pages, v_pages, k_scales, v_scales, block_table, kv_
     out = _out(call, out, q, "out")
     lse = call.empty(q, q.shape[:3], N.LC_DTYPE_F32) if return_lse else None
     ws = call.workspace(nbytes)
-    _check(_lib().lcKvCacheAttention(
-        _byref(c), cfg, _tensor4(call, q, "q"), call.addr(t), stride, _addr(call, lengths), _tensor4(call, out, "out"),
-        _addr(call, lse), _addr(call, ws), nbytes, call.stream))
+    call.run("lcKvCacheAttention", "iitpiptppii",
+             (ctypes.addressof(c), cfg.at, q, t, stride, lengths, out, lse, ws, nbytes, call.stream), "q out")
     got = call.finish(out, lse)
     return got if return_lse else got[0]

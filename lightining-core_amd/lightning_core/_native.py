@@ -241,19 +241,19 @@ SIGNATURES = {
     "lcHipDeviceIndex": (_E, [P(c_int)]),
     "lcHipBackendStream": (_E, [P(c_void_p)]),
     "lcCrossAttentionWorkspaceSize": (_E, [P(CrossAttentionConfig), c_int, P(c_size)]),
-    "lcCrossAttentionForward": (_E, [P(CrossAttentionConfig)] + [P(DeviceTensor)] * 3 + [BUF, P(DeviceTensor), BUF, BUF,
+    "lcCrossAttentionForward": (_E, [BUF] + [P(DeviceTensor)] * 3 + [BUF, P(DeviceTensor), BUF, BUF,
                                                                                        c_size, c_void_p]),
-    "lcCrossAttentionBackward": (_E, [P(CrossAttentionConfig)] + [P(DeviceTensor)] * 5 + [BUF, BUF]
+    "lcCrossAttentionBackward": (_E, [BUF] + [P(DeviceTensor)] * 5 + [BUF, BUF]
                                  + [P(DeviceTensor)] * 3 + [BUF, c_size, c_void_p]),
     "lcLayerNormWorkspaceSize": (_E, [P(LayerNormConfig), P(c_size)]),
-    "lcLayerNormForward": (_E, [P(LayerNormConfig), BUF, ctypes.c_int64, BUF, BUF, BUF, ctypes.c_int64, BUF, BUF,
+    "lcLayerNormForward": (_E, [BUF, BUF, ctypes.c_int64, BUF, BUF, BUF, ctypes.c_int64, BUF, BUF,
                                 c_void_p]),
-    "lcLayerNormBackward": (_E, [P(LayerNormConfig), BUF, ctypes.c_int64, BUF, ctypes.c_int64, BUF, BUF, BUF, BUF,
+    "lcLayerNormBackward": (_E, [BUF, BUF, ctypes.c_int64, BUF, ctypes.c_int64, BUF, BUF, BUF, BUF,
                                  ctypes.c_int64, BUF, BUF, BUF, c_size, c_void_p]),
-    "lcKvCacheStore": (_E, [P(KvCache), c_size, c_size, c_int, P(DeviceTensor), P(DeviceTensor), BUF, c_size,
+    "lcKvCacheStore": (_E, [BUF, c_size, c_size, c_int, P(DeviceTensor), P(DeviceTensor), BUF, c_size,
                             ctypes.c_int64, BUF, c_void_p]),
     "lcKvCacheAttentionWorkspaceSize": (_E, [P(KvCache), P(KvAttentionConfig), P(c_size)]),
-    "lcKvCacheAttention": (_E, [P(KvCache), P(KvAttentionConfig), P(DeviceTensor), BUF, ctypes.c_int64, BUF,
+    "lcKvCacheAttention": (_E, [BUF, BUF, P(DeviceTensor), BUF, ctypes.c_int64, BUF,
                                 P(DeviceTensor), BUF, BUF, c_size, c_void_p]),
     "lcHipGetDeviceInfo": (_E, [P(HipDeviceInfo)]),
     "lcHipTimerCreate": (_E, [P(c_void_p)]),
