@@ -122,3 +122,32 @@ def test_both_routes_refuse_alike(monkeypatch, compiled):
     wide = torch.zeros(1, 2, 3, 1000, device="cuda")  # a head size that the library refuses
     with pytest.raises(RuntimeError):
         lc.cross_attention(wide, wide, wide)
+
+
+@pytest.mark.gpu
+def test_threads_on_streams_of_their_own():
+    """Two threads call at once, each on its own stream; the results are the bits of one alone."""
+    import threading
+    want = _calls()
+    torch.cuda.synchronize()
+    got, errors = [[], []], []
+
+    def work(i):
+        try:
+            stream = torch.cuda.Stream()
+            with torch.cuda.stream(stream):
+                for _ in range(10):
+                    got[i].append(_calls())
+                stream.synchronize()
+        except Exception as e:  # shown by the assertion below
+            errors.append(e)
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors
+    for results in got:
+        assert len(results) == 10
+        for r in results:
+            assert all(torch.equal(x, y) for x, y in zip(r, want))
