@@ -20,10 +20,6 @@ import sys
 
 import torch
 
-_PKG = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "lightining-core_amd")
-if _PKG not in sys.path:
-    sys.path.insert(0, _PKG)
-
 own = False
 
 PAGE = 64
@@ -32,6 +28,9 @@ _GPU = "cuda"
 
 
 def _lc():
+    pkg = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "lightining-core_amd")
+    if pkg not in sys.path:
+        sys.path.insert(0, pkg)
     import lightning_core
 
     return lightning_core
