@@ -346,7 +346,7 @@ struct XTensor {
 struct XAttnArgs {
   XTensor q, k, v, o, go, dq, dk, dv;  // backward: o and go (dO) are read
   float* lse;                          // [batch, heads, q_len]; the forward's may be null
-  float* delta;                        // backward: [batch, heads, q_len][2]
+  float* delta;                        // backward: [batch, heads, q_len][2], delta and lse * log2(e)
   const int32_t* lengths;              // [batch] keys of each batch row, or null (all kv_len)
   int batch, heads, kv_heads, q_len, kv_len, d;
   float c;      // |scale| * log2(e); `negate` when scale < 0

@@ -768,19 +768,54 @@ __global__ __launch_bounds__(256) void xattn_join_kernel(XAttnArgs a) {
 }
 
 // ---------------------------------------------------------------------------
-// fp16 gradients: dS can be far below fp16's range (dO carries no fixed scale,
-// and P shares one among thousands of keys), so it is rounded with dO's rows
-// scaled by a power of two to a largest value in [1/8, 1/4), and the gradient
-// is scaled back at the end.  |dS| <= 2 d / 4 max|V| then stays inside the type
-// for values up to 1000.
-constexpr int kNoExponent = -126;  // a row of zeros: it sets no scale
-__device__ __forceinline__ int exponent_of(float amax) {
-  // Infinities and NaN stay what they are at any scale.
-  return amax > 0.0f ? (amax < INFINITY ? __builtin_amdgcn_frexp_expf(amax) + 2 : 0) : kNoExponent;
-}
-__device__ __forceinline__ float power_of_two(int e) { return __builtin_amdgcn_ldexpf(1.0f, e); }
+// fp16 gradients: dS goes to fp16 for the matrix cores, and nothing bounds it
+// on either side (dO carries no fixed scale, V may be large, and P shares one
+// among thousands of keys).  dQ's accumulators belong to one query row a lane
+// and dK's to one key, so each lane holds its own at a power of two, 2^e, of the
+// true gradient: the first block's largest |dS| of the row or key comes to
+// [2^7, 2^8), and e falls when a later one would pass 2^15.  What the largest
+// value so far leaves normal reaches down to 2^-21 of it.  (A scale from dO
+// alone lets dS overflow for large V: two keys of 20000 and 0, 128 columns.)
+// 64 heads of 2048 x 1500 x 128: 408 us, bf16 without it 372.
+struct Lift {
+  int e = 126;               // nothing seen: values below 2^-111 pass as they are
+  float up = 0x1p126f;       // 2^e
+  float most = 0x1p-111f;    // 2^(15 - e)
+  // ds *= 2^e for the lane's e, after `acc` has followed e.  `on`: the lane's
+  // column is one whose gradient is kept.
+  template <int DT>
+  __device__ __forceinline__ void apply(floatx16& ds, bool on, floatx16 (&acc)[DT]) {
+    float top = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      top = fmaxf(top, fabsf(ds[i]));
+    }
+    top = max_xor32(top);
+    top = on ? top : 0.0f;
+    if (__any(top >= most)) {
+      const int next = top >= most ? 8 - __builtin_amdgcn_frexp_expf(top) : e;
+      const float f = __builtin_amdgcn_ldexpf(1.0f, next - e);
+      e = next;
+      up = __builtin_amdgcn_ldexpf(1.0f, e);
+      most = __builtin_amdgcn_ldexpf(1.0f, 15 - e);
+#pragma unroll
+      for (int t = 0; t < DT; ++t) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          acc[t][i] *= f;
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      ds[i] *= up;
+    }
+  }
+  // 2^-e, by which the gradient is scaled back.
+  __device__ __forceinline__ float down() const { return __builtin_amdgcn_ldexpf(1.0f, -e); }
+};
 
-// Each query row's delta = dO . O and the exponent of its dO, 16 threads a row.
+// Each query row's delta = dO . O, and its lse in exp2 units, 16 threads a row.
 template <typename T, bool VEC>
 __global__ __launch_bounds__(256) void xattn_delta_kernel(XAttnArgs a) {
   using E = typename Elem<T>::type;
@@ -795,7 +830,6 @@ __global__ __launch_bounds__(256) void xattn_delta_kernel(XAttnArgs a) {
   const E* g = static_cast<const E*>(a.go.p) + b * a.go.sb + h * a.go.sh + pos * a.go.ss;
   const E* o = static_cast<const E*>(a.o.p) + b * a.o.sb + h * a.o.sh + pos * a.o.ss;
   float delta = 0.0f;
-  float amax = 0.0f;
 #pragma unroll
   for (int j = 0; j < kern::kXAttnMaxDim / (16 * EC); ++j) {
     const int c = (threadIdx.x & 15) + 16 * j;
@@ -804,22 +838,20 @@ __global__ __launch_bounds__(256) void xattn_delta_kernel(XAttnArgs a) {
 #pragma unroll
     for (int i = 0; i < EC; ++i) {
       delta = fmaf(chunk_value<T>(gv, i), chunk_value<T>(ov, i), delta);
-      amax = fmaxf(amax, fabsf(chunk_value<T>(gv, i)));
     }
   }
 #pragma unroll
   for (int x = 8; x > 0; x >>= 1) {
     delta += __shfl_xor(delta, x);
-    amax = fmaxf(amax, __shfl_xor(amax, x));
   }
   if ((threadIdx.x & 15) == 0 && row < rows) {
-    *reinterpret_cast<float2*>(a.delta + 2 * row) = make_float2(delta, static_cast<float>(exponent_of(amax)));
+    *reinterpret_cast<float2*>(a.delta + 2 * row) = make_float2(delta, a.lse[row] * kLog2e);
   }
 }
 
 // dQ of 128 rows (block `blk`) over share z of the keys: as the forward, with
 // dO's rows beside Q's.  DELTA: the rows' delta = sum over the keys of P dP
-// instead (of all keys, splits_q being ignored), with the exponent of dO.
+// instead (of all keys, splits_q being ignored).
 template <typename T, int DP, bool VEC, bool DELTA>
 __device__ __forceinline__ void dq_part(const XAttnArgs& a, char* smem, int blk, int z) {
   using TL = Tile<T, DP>;
@@ -862,17 +894,17 @@ __device__ __forceinline__ void dq_part(const XAttnArgs& a, char* smem, int blk,
     }
   }
   const size_t lrow = (static_cast<size_t>(b) * a.heads + qr.head) * a.q_len + qr.pos;
-  const float lse2 = valid ? a.lse[lrow] * kLog2e : 0.0f;
-  float2 de = make_float2(0.0f, 0.0f);
-  if (!DELTA && valid) {
-    de = *reinterpret_cast<const float2*>(a.delta + 2 * lrow);
+  float2 st = make_float2(0.0f, 0.0f);
+  if (valid) {
+    if constexpr (DELTA) {
+      st.y = a.lse[lrow] * kLog2e;
+    } else {
+      st = *reinterpret_cast<const float2*>(a.delta + 2 * lrow);
+    }
   }
-  const float delta = de.x;
-  const int ex = static_cast<int>(de.y);
-  float down = 1.0f;
-  if constexpr (__is_same(T, F16) && !DELTA) {
-    down = power_of_two(-ex);
-  }
+  const float delta = st.x;
+  const float lse2 = st.y;
+  Lift lift;  // fp16
   float sum = 0.0f;
   floatx16 dq[TL::DT];
 #pragma unroll
@@ -905,7 +937,7 @@ __device__ __forceinline__ void dq_part(const XAttnArgs& a, char* smem, int blk,
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         const float p = fast_exp2(fmaf(s[i], c, -lse2));
-        s[i] = DELTA ? p * dp[i] : p * (dp[i] - delta) * down;
+        s[i] = DELTA ? p * dp[i] : p * (dp[i] - delta);
       }
       if (tail) {
 #pragma unroll
@@ -921,6 +953,9 @@ __device__ __forceinline__ void dq_part(const XAttnArgs& a, char* smem, int blk,
           sum += s[i];
         }
       } else if constexpr (TL::EC == 8) {
+        if constexpr (__is_same(T, F16)) {
+          lift.apply(s, valid, dq);
+        }
         u32x4 pk[2];
         pack_block<T>(s, pk);
         __builtin_amdgcn_s_setprio(1);
@@ -933,18 +968,9 @@ __device__ __forceinline__ void dq_part(const XAttnArgs& a, char* smem, int blk,
     arrive();
   }
   if constexpr (DELTA) {
-    float amax = 0.0f;
-#pragma unroll
-    for (int x = 0; x < TL::NS; ++x) {
-#pragma unroll
-      for (int i = 0; i < TL::EC; ++i) {
-        amax = fmaxf(amax, fabsf(chunk_value<T>(gf[x], i)));
-      }
-    }
     sum = add_xor32(sum);
-    amax = max_xor32(amax);
     if (valid && half == 0) {
-      *reinterpret_cast<float2*>(a.delta + 2 * lrow) = make_float2(sum, static_cast<float>(exponent_of(amax)));
+      *reinterpret_cast<float2*>(a.delta + 2 * lrow) = make_float2(sum, lse2);
     }
     return;
   }
@@ -955,7 +981,7 @@ __device__ __forceinline__ void dq_part(const XAttnArgs& a, char* smem, int blk,
   // difference between dP and delta.
   float f = len > 1 ? a.scale : 0.0f;
   if constexpr (__is_same(T, F16)) {
-    f *= power_of_two(ex);
+    f *= lift.down();
   }
   if (a.splits_q > 1) {
     const size_t prow = (static_cast<size_t>(z) * gridDim.x + blockIdx.x) * R + r;
@@ -969,7 +995,7 @@ __device__ __forceinline__ void dq_part(const XAttnArgs& a, char* smem, int blk,
 constexpr int kQueryTile = 32;
 template <typename T, int DP>
 constexpr size_t dkv_lds_bytes() {
-  return (4 * kQueryTile + 128) * Tile<T, DP>::RB + 6 * kQueryTile * sizeof(float);
+  return (4 * kQueryTile + 128) * Tile<T, DP>::RB + 4 * kQueryTile * sizeof(float);
 }
 
 // dK and dV of 128 keys (block `blk`), four waves of 32, over share z of the
@@ -983,9 +1009,9 @@ __device__ __forceinline__ void dkv_part(const XAttnArgs& a, char* smem, int blk
   using E = typename Elem<T>::type;
   constexpr int KT = kQueryTile;
   constexpr int TB = KT * TL::RB;
-  // LDS: Q and dO tiles, then lse, delta and exponents, then V.
-  float* const st = reinterpret_cast<float*>(smem + 4 * TB);   // [2][3][KT]
-  char* const own = smem + 4 * TB + 6 * KT * sizeof(float);
+  // LDS: Q and dO tiles, then lse and delta, then V.
+  float* const st = reinterpret_cast<float*>(smem + 4 * TB);   // [2][2][KT]
+  char* const own = smem + 4 * TB + 4 * KT * sizeof(float);
   const int tid = threadIdx.x;
   const int lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -1004,7 +1030,7 @@ __device__ __forceinline__ void dkv_part(const XAttnArgs& a, char* smem, int blk
   Stream<T, DP, KT, VEC, 4> qs, gs;
   qs.init(a.q.p, a.q.ss, a.q_len, a.d, wave, lane);
   gs.init(a.go.p, a.go.ss, a.q_len, a.d, wave, lane);
-  float rl = 0.0f, rd = 0.0f, re = 0.0f;
+  float rl = 0.0f, rd = 0.0f;
   // Starts moving tile t; its rows' statistics stay in registers until `keep`.
   auto stage = [&](int t, int buf) {
     const int g = t / per_head;
@@ -1016,9 +1042,8 @@ __device__ __forceinline__ void dkv_part(const XAttnArgs& a, char* smem, int blk
       const size_t row = (static_cast<size_t>(b) * a.heads + head) * a.q_len + (in ? pos : 0);
       const float* dr = a.delta + 2 * row;
       // A row past the end has probabilities of zero.
-      rl = in ? a.lse[row] * kLog2e : INFINITY;
+      rl = in ? dr[1] : INFINITY;
       rd = in ? dr[0] : 0.0f;
-      re = in ? dr[1] : kNoExponent;
     }
     qs.rebase(static_cast<const E*>(a.q.p) + b * a.q.sb + head * a.q.sh);
     gs.rebase(static_cast<const E*>(a.go.p) + b * a.go.sb + head * a.go.sh);
@@ -1027,10 +1052,9 @@ __device__ __forceinline__ void dkv_part(const XAttnArgs& a, char* smem, int blk
   };
   auto keep = [&](int buf) {
     if (tid < KT) {
-      float* sl = st + buf * 3 * KT;
+      float* sl = st + buf * 2 * KT;
       sl[tid] = rl;
       sl[KT + tid] = rd;
-      sl[2 * KT + tid] = re;
     }
   };
   u32x4 kf[TL::NS];
@@ -1056,7 +1080,7 @@ __device__ __forceinline__ void dkv_part(const XAttnArgs& a, char* smem, int blk
     dk[t] = zero16();
     dv[t] = zero16();
   }
-  int ex = kNoExponent;  // fp16: dk is held at 2^-ex
+  Lift lift;  // fp16
   const float c = a.c;
   if (t0 < t1) {
     keep(0);
@@ -1066,30 +1090,9 @@ __device__ __forceinline__ void dkv_part(const XAttnArgs& a, char* smem, int blk
     const int buf = (t - t0) & 1;
     const char* ql = smem + buf * TB;
     const char* gl = ql + 2 * TB;
-    const float* sl = st + buf * 3 * KT;
+    const float* sl = st + buf * 2 * KT;
     if (t + 1 < t1) {
       stage(t + 1, 1 - buf);
-    }
-    float down = 1.0f;
-    if constexpr (__is_same(T, F16)) {
-      float e = sl[2 * KT + (lane & (KT - 1))];
-#pragma unroll
-      for (int x = KT / 2; x > 0; x >>= 1) {
-        e = fmaxf(e, __shfl_xor(e, x));
-      }
-      const int et = __builtin_amdgcn_readfirstlane(static_cast<int>(e));
-      if (et > ex) {
-        const float f = power_of_two(ex - et);
-        ex = et;
-#pragma unroll
-        for (int t2 = 0; t2 < TL::DT; ++t2) {
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            dk[t2][i] *= f;
-          }
-        }
-      }
-      down = power_of_two(-ex);
     }
     floatx16 s = zero16();
     floatx16 dp = zero16();
@@ -1109,7 +1112,7 @@ __device__ __forceinline__ void dkv_part(const XAttnArgs& a, char* smem, int blk
       for (int i = 0; i < 4; ++i) {
         const float p = fast_exp2(fmaf(s[4 * g + i], c, -lv[i]));
         s[4 * g + i] = p;
-        dp[4 * g + i] = p * (dp[4 * g + i] - dl[i]) * down;
+        dp[4 * g + i] = p * (dp[4 * g + i] - dl[i]);
       }
     }
     if constexpr (TL::EC == 8) {
@@ -1118,6 +1121,9 @@ __device__ __forceinline__ void dkv_part(const XAttnArgs& a, char* smem, int blk
       // As in the forward: 383 -> 375 us for the whole pass at 2048 x 1500.
       __builtin_amdgcn_s_setprio(1);
       TL::transposed(gl, 0, pk, lane, dv);
+      if constexpr (__is_same(T, F16)) {
+        lift.apply(dp, valid, dk);
+      }
       u32x4 pd[2];
       pack_block<T>(dp, pd);
       TL::transposed(ql, 0, pd, lane, dk);
@@ -1138,7 +1144,7 @@ __device__ __forceinline__ void dkv_part(const XAttnArgs& a, char* smem, int blk
   float fk = valid && len > 1 ? a.scale : 0.0f;
   const float fv = valid ? 1.0f : 0.0f;
   if constexpr (__is_same(T, F16)) {
-    fk *= power_of_two(ex);
+    fk *= lift.down();
   }
   if (!valid) {
 #pragma unroll
