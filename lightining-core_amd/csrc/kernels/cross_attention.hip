@@ -998,6 +998,13 @@ constexpr size_t dkv_lds_bytes() {
   return (4 * kQueryTile + 128) * Tile<T, DP>::RB + 4 * kQueryTile * sizeof(float);
 }
 
+// fp16: P goes to fp16 as 2^15 P, at most half its largest number, so that it is
+// normal down to 2^-29 (as P alone to 2^-14: among 16384 keys most are not).
+template <typename T>
+constexpr int probability_lift() {
+  return __is_same(T, F16) ? 15 : 0;
+}
+
 // dK and dV of 128 keys (block `blk`), four waves of 32, over share z of the
 // query tiles; Q and dO stream.  The workgroup's own rows of V stay in LDS: in
 // registers beside K's and two accumulators they would leave room for one wave
@@ -1042,7 +1049,7 @@ __device__ __forceinline__ void dkv_part(const XAttnArgs& a, char* smem, int blk
       const size_t row = (static_cast<size_t>(b) * a.heads + head) * a.q_len + (in ? pos : 0);
       const float* dr = a.delta + 2 * row;
       // A row past the end has probabilities of zero.
-      rl = in ? dr[1] : INFINITY;
+      rl = in ? dr[1] - probability_lift<T>() : INFINITY;
       rd = in ? dr[0] : 0.0f;
     }
     qs.rebase(static_cast<const E*>(a.q.p) + b * a.q.sb + head * a.q.sh);
@@ -1142,9 +1149,11 @@ __device__ __forceinline__ void dkv_part(const XAttnArgs& a, char* smem, int blk
   }
   // Keys past the row's length have gradients of zero.
   float fk = valid && len > 1 ? a.scale : 0.0f;
-  const float fv = valid ? 1.0f : 0.0f;
+  float fv = valid ? 1.0f : 0.0f;
   if constexpr (__is_same(T, F16)) {
-    fk *= lift.down();
+    constexpr float kDown = 1.0f / (1 << probability_lift<T>());
+    fk *= lift.down() * kDown;
+    fv *= kDown;
   }
   if (!valid) {
 #pragma unroll

@@ -111,3 +111,9 @@ def test_many_keys_dk(lc):
     got, want, rows, _ = _many_keys(lc)
     bound = want[1].abs() * (2 * STEP + E_P + rows * F) * 1.01
     assert_within(got[1], want[1], bound + 2.0**-25, "dk")
+
+
+def test_many_keys_dv(lc):
+    got, want, rows, _ = _many_keys(lc)
+    bound = want[2].abs() * (2 * STEP + E_P + rows * F) * 1.01
+    assert_within(got[2], want[2], bound + 2.0**-25, "dv")
