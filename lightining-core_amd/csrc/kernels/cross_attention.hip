@@ -349,11 +349,15 @@ constexpr int waves_per_simd() {
 // The softmax state of a wave's 32 query rows (one a lane, in both lane halves)
 // over tiles of KT keys.  Scores and m in exp2 units.  m follows the running
 // maximum lazily: O and l are rescaled only when a tile's maximum passes it by
-// more than 8 (probabilities up to 256).
+// more than 8 (probabilities up to 256).  fp16: m is 7 below the maximum it was
+// taken from, so that P, which goes to fp16, lies between 2^7 and 2^15 at its
+// largest and is normal down to 2^-21 of that: a tail of very many keys far
+// below the maximum, whose values count together, keeps its bits.
 template <typename T, int DP, int KT>
 struct FwdState {
   using TL = Tile<T, DP>;
   static constexpr int NB = KT / 32;
+  static constexpr float kBelow = __is_same(T, F16) ? 7.0f : 0.0f;
   u32x4 qf[TL::NS];
   floatx16 o[TL::DT];
   float m;
@@ -405,7 +409,7 @@ struct FwdState {
         top = fmaxf(top, s[n][i]);
       }
     }
-    top = max_xor32(top) * c;
+    top = fmaf(max_xor32(top), c, -kBelow);
     if (__any(top > m + 8.0f)) {
       const float next = fmaxf(m, top);
       const float f = m == -INFINITY ? 0.0f : fast_exp2(m - next);

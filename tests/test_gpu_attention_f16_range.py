@@ -117,3 +117,28 @@ def test_many_keys_dv(lc):
     got, want, rows, _ = _many_keys(lc)
     bound = want[2].abs() * (2 * STEP + E_P + rows * F) * 1.01
     assert_within(got[2], want[2], bound + 2.0**-25, "dv")
+
+
+@pytest.mark.parametrize("rows,score", [(3, 11.75), (65536, 14.25)])
+def test_many_keys_far_below_one(lc, rows, score):
+    """One key whose score is far above those of 65536 equal ones: half of the
+    columns are theirs alone.  Few rows: each wave has some of the keys; many: all."""
+    keys, d = 65537, 64
+    q, k, v = (torch.zeros((1, 1, n, d)) for n in (rows, keys, keys))
+    q[..., 0], k[..., 0, 0] = 8.0, score
+    v[..., 1:, :32], v[..., 0, 32:] = 1.0, 1.0
+    q, k, v = (x.to(HALF).cuda() for x in (q, k, v))
+    print("[case] one key above many", flush=True)
+    out, lse = lc.cross_attention(q, k, v, return_lse=True)
+    torch.cuda.synchronize()
+    rest = (keys - 1) * math.exp(-score)
+    total = 1 + rest
+    want = torch.full(out.shape, 1 / total, dtype=torch.float64, device="cuda")
+    want[..., :32] = rest / total
+    # P and the result rounded to fp16; the score in exp2 units and the
+    # exponential.  A lane adds up at most half the keys for l, and a wave's
+    # products all of them, 16 to an instruction with at most two roundings.
+    e_sum = (keys / 2 + keys / 8 + 64) * F
+    assert_within(out, want, want * (2 * STEP + e_sum) * 1.01, "out")
+    assert_within(lse, torch.full(lse.shape, score + math.log(total), dtype=torch.float64, device="cuda"),
+                  torch.full(lse.shape, e_sum, dtype=torch.float64, device="cuda"), "lse")
