@@ -370,7 +370,7 @@ constexpr int kXAttnRows = 128;  // rows (or keys) of a workgroup
 constexpr int kXAttnMaxDim = 128;
 constexpr int kXAttnWidth(int d) { return d <= 64 ? 64 : 128; }
 constexpr int kXAttnFewRows = 32;
-constexpr int kXAttnShortKeys = 128;  // 16-bit backward: delta from the probabilities
+constexpr int kXAttnShortKeys = 128;  // 16-bit backward: delta from the probabilities of a row's own keys
 constexpr int kXAttnTile(DType t) { return t == DType::kF32 ? 32 : 64; }  // keys
 constexpr int kXAttnQueryTile = 32;                                       // queries, for dK and dV
 // `aligned`: every tensor's base is 16-byte aligned, its strides and d are

@@ -819,37 +819,61 @@ struct Lift {
   __device__ __forceinline__ float down() const { return __builtin_amdgcn_ldexpf(1.0f, -e); }
 };
 
-// Each query row's delta = dO . O, and its lse in exp2 units, 16 threads a row.
-template <typename T, bool VEC>
-__global__ __launch_bounds__(256) void xattn_delta_kernel(XAttnArgs a) {
+// The statistics of ROWS query rows (block `blk`): delta = dO . O and lse in exp2
+// units, 16 threads a row.  All loads are issued before the first is used: few
+// workgroups run at once beside the LDS that short rows need.
+template <typename T, bool VEC, int ROWS>
+__device__ __forceinline__ void delta_rows(const XAttnArgs& a, int blk) {
   using E = typename Elem<T>::type;
   constexpr int EC = Elem<T>::kChunk;
-  const size_t rows = static_cast<size_t>(a.batch) * a.heads * a.q_len;
-  const size_t row = static_cast<size_t>(blockIdx.x) * 16 + (threadIdx.x >> 4);
-  const size_t at = row < rows ? row : 0;
-  const size_t head = at / a.q_len;
-  const int64_t pos = static_cast<int64_t>(at - head * a.q_len);
-  const int64_t b = static_cast<int64_t>(head / a.heads);
-  const int64_t h = static_cast<int64_t>(head - b * a.heads);
-  const E* g = static_cast<const E*>(a.go.p) + b * a.go.sb + h * a.go.sh + pos * a.go.ss;
-  const E* o = static_cast<const E*>(a.o.p) + b * a.o.sb + h * a.o.sh + pos * a.o.ss;
-  float delta = 0.0f;
+  constexpr int N = ROWS / 16;
+  constexpr int NC = kern::kXAttnMaxDim / (16 * EC);
+  const int b = blockIdx.x / a.kv_heads;
+  const int hk = blockIdx.x - b * a.kv_heads;
+  const int group = a.heads / a.kv_heads;
+  const int R = group * a.q_len;
+  const int r0 = blk * ROWS + static_cast<int>(threadIdx.x >> 4);
+  u32x4 gv[N][NC], ov[N][NC];
+  size_t row[N];
+  float lse[N];
 #pragma unroll
-  for (int j = 0; j < kern::kXAttnMaxDim / (16 * EC); ++j) {
-    const int c = (threadIdx.x & 15) + 16 * j;
-    const u32x4 gv = load_chunk<T, VEC>(g, c, a.d);
-    const u32x4 ov = load_chunk<T, VEC>(o, c, a.d);
+  for (int n = 0; n < N; ++n) {
+    const bool in = r0 + 16 * n < R;
+    const QueryRow qr = query_row(in ? r0 + 16 * n : 0, a.q_len, hk * group);
+    const int64_t pos = qr.pos;
+    const E* g = static_cast<const E*>(a.go.p) + b * a.go.sb + qr.head * a.go.sh + pos * a.go.ss;
+    const E* o = static_cast<const E*>(a.o.p) + b * a.o.sb + qr.head * a.o.sh + pos * a.o.ss;
+    row[n] = (static_cast<size_t>(b) * a.heads + qr.head) * a.q_len + qr.pos;
 #pragma unroll
-    for (int i = 0; i < EC; ++i) {
-      delta = fmaf(chunk_value<T>(gv, i), chunk_value<T>(ov, i), delta);
+    for (int j = 0; j < NC; ++j) {
+      const int c = (threadIdx.x & 15) + 16 * j;
+      if constexpr (VEC) {
+        gv[n][j] = load_chunk_flat(g, c * 16, a.d * static_cast<int>(sizeof(E)), in);
+        ov[n][j] = load_chunk_flat(o, c * 16, a.d * static_cast<int>(sizeof(E)), in);
+      } else {
+        gv[n][j] = load_chunk<T, VEC>(g, c, a.d);
+        ov[n][j] = load_chunk<T, VEC>(o, c, a.d);
+      }
     }
+    lse[n] = a.lse[row[n]];
   }
 #pragma unroll
-  for (int x = 8; x > 0; x >>= 1) {
-    delta += __shfl_xor(delta, x);
-  }
-  if ((threadIdx.x & 15) == 0 && row < rows) {
-    *reinterpret_cast<float2*>(a.delta + 2 * row) = make_float2(delta, a.lse[row] * kLog2e);
+  for (int n = 0; n < N; ++n) {
+    float delta = 0.0f;
+#pragma unroll
+    for (int j = 0; j < NC; ++j) {
+#pragma unroll
+      for (int i = 0; i < EC; ++i) {
+        delta = fmaf(chunk_value<T>(gv[n][j], i), chunk_value<T>(ov[n][j], i), delta);
+      }
+    }
+#pragma unroll
+    for (int x = 8; x > 0; x >>= 1) {
+      delta += __shfl_xor(delta, x);
+    }
+    if ((threadIdx.x & 15) == 0 && r0 + 16 * n < R) {
+      *reinterpret_cast<float2*>(a.delta + 2 * row[n]) = make_float2(delta, lse[n] * kLog2e);
+    }
   }
 }
 
@@ -1195,14 +1219,33 @@ __global__ __launch_bounds__(256, (VEC && (Elem<T>::kChunk == 8 || DP == 64) ? 2
   }
 }
 
-// delta from the probabilities instead of from `out`: grid (problems, row
-// blocks).  A 16-bit `out` has lost 2^-9 of itself, and with few keys it is of
-// the values' own size: dQ and dK of 18 keys were 1.7 times as far from 64 bits
-// as a rounding of the exact ones is.  Two more products, for short keys only.
+// Parts of a 128-row block, a workgroup each, where delta comes from `out`: fp32;
+// 16-bit types whose blocks would not fill the chip (else one).
+constexpr int kDeltaParts = 8;
+constexpr int kDeltaPartsFew = 4;
+
+// Every query row's delta: grid (problems, 128-row blocks, parts).  16-bit
+// types take it from the probabilities instead of from `out` where the batch row
+// has few keys of its own, however far it is padded: a 16-bit `out` has lost 2^-9
+// of itself, and with few keys it is of the values' own size (dQ and dK of 18
+// keys were 1.7 times as far from 64 bits as a rounding of the exact ones is).
+// Two more products, for short keys only.  us, one kernel for either kind of
+// row: 64 heads of 2048 rows of 128 from `out` 15 (a kernel without LDS 14), 64
+// heads of 512 x 100 x 64 from the probabilities 6.7.
 template <typename T, int DP, bool VEC>
-__global__ __launch_bounds__(256, (waves_per_simd<T, DP, VEC>())) void xattn_delta_keys_kernel(XAttnArgs a) {
+__global__ __launch_bounds__(256, (waves_per_simd<T, DP, VEC>())) void xattn_delta_kernel(XAttnArgs a) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  dq_part<T, DP, VEC, true>(a, smem, blockIdx.y, 0);
+  if constexpr (Elem<T>::kChunk == 4) {
+    delta_rows<T, VEC, 128 / kDeltaParts>(a, blockIdx.y * kDeltaParts + blockIdx.z);
+  } else if (keys_of(a, blockIdx.x / a.kv_heads) <= kern::kXAttnShortKeys) {
+    if (blockIdx.z == 0) {
+      dq_part<T, DP, VEC, true>(a, smem, blockIdx.y, 0);
+    }
+  } else if (gridDim.z == 1) {
+    delta_rows<T, VEC, 128>(a, blockIdx.y);
+  } else {
+    delta_rows<T, VEC, 128 / kDeltaPartsFew>(a, blockIdx.y * kDeltaPartsFew + blockIdx.z);
+  }
 }
 
 // Sums the shares' partial rows in their order, a wave per row: blockIdx.y 0 dQ
@@ -1283,18 +1326,16 @@ hipError_t launch_backward(const XAttnArgs& a, hipStream_t stream) {
   const size_t rows_q = static_cast<size_t>(a.batch) * a.heads * a.q_len;
   const size_t rows_kv = static_cast<size_t>(a.batch) * a.kv_heads * a.kv_len;
   const unsigned q_blocks = static_cast<unsigned>((a.heads / a.kv_heads * a.q_len + 127) / 128);
-  constexpr bool k16 = Elem<T>::kChunk == 8;
-  if (k16 && rows_q != 0 && a.kv_len <= kern::kXAttnShortKeys) {
-    constexpr size_t lds = tiles_bytes<T, DP>();
-    static const hipError_t allowed = LC_XATTN_ALLOW((xattn_delta_keys_kernel<T, DP, VEC>), lds);
-    const hipError_t e = launch_lds(xattn_delta_keys_kernel<T, DP, VEC>, allowed,
-                                    dim3(static_cast<unsigned>(a.batch * a.kv_heads), q_blocks), lds, a, stream);
-    if (e != hipSuccess) {
-      return e;
-    }
-  } else if (rows_q != 0) {
-    xattn_delta_kernel<T, VEC><<<static_cast<unsigned>((rows_q + 15) / 16), 256, 0, stream>>>(a);
-    const hipError_t e = hipGetLastError();
+  const unsigned problems = static_cast<unsigned>(a.batch * a.kv_heads);
+  if (rows_q != 0) {
+    constexpr bool k16 = Elem<T>::kChunk == 8;
+    // LDS where a row may take delta from the probabilities.
+    constexpr size_t most = k16 ? tiles_bytes<T, DP>() : 0;
+    const size_t lds = a.lengths != nullptr || a.kv_len <= kern::kXAttnShortKeys ? most : 0;
+    static const hipError_t allowed = LC_XATTN_ALLOW((xattn_delta_kernel<T, DP, VEC>), most);
+    // A workgroup for each CU at least (2 x 2 heads of keys, 308 rows each: 5.1 -> 3.3 us).
+    const dim3 grid(problems, q_blocks, !k16 ? kDeltaParts : problems * q_blocks < 256 ? kDeltaPartsFew : 1);
+    const hipError_t e = launch_lds(xattn_delta_kernel<T, DP, VEC>, allowed, grid, lds, a, stream);
     if (e != hipSuccess) {
       return e;
     }

@@ -1,0 +1,58 @@
+"""16-bit cross attention gradients of a row do not depend on how far the other
+rows pad the batch: up to 128 keys of its own, delta comes from the probabilities.
+"""
+import pytest
+import torch
+
+from decoder_ref import U, Attention, assert_within
+from gpu_util import require_hip
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def lc():
+    return require_hip()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("d", [64, 128, 40])
+@pytest.mark.parametrize("sq", [1, 50, 300])
+def test_padding_changes_nothing(lc, dtype, d, sq):
+    gen = torch.Generator()
+    gen.manual_seed(d + sq)
+    lens, keys, hq, hkv = [18, 2, 64, 1, 0, 128, 100], 128, 4, 2
+    b = len(lens)
+    q, dout = (torch.randn((b, hq, sq, d), generator=gen).to(dtype).cuda() for _ in range(2))
+    k, v = (torch.randn((b, hkv, keys, d), generator=gen).to(dtype).cuda() for _ in range(2))
+    lengths = torch.tensor(lens, dtype=torch.int32, device="cuda")
+
+    def run(pad, longer):
+        """The batch padded to `pad`, with a row that is that long when `longer`."""
+        extra = 1 if longer else 0
+        x = [torch.randn((b + extra, t.shape[1], n, d), generator=gen).to(dtype).cuda()
+             for t, n in ((dout, sq), (q, sq), (k, pad), (v, pad))]
+        for y, t in zip(x, (dout, q, k, v)):
+            y[:b, :, :t.shape[2]] = t
+        n = torch.cat([lengths, torch.tensor([pad] * extra, dtype=torch.int32, device="cuda")])
+        print(f"[case] {dtype} d={d} sq={sq} padded to {pad}", flush=True)
+        out, lse = lc.cross_attention(x[1], x[2], x[3], n, return_lse=True)
+        dq, dk, dv = lc.cross_attention_backward(x[0], *x[1:], out, lse, n)
+        torch.cuda.synchronize()
+        assert (dk[:b, :, keys:] == 0).all() and (dv[:b, :, keys:] == 0).all()
+        return dq[:b], dk[:b, :, :keys], dv[:b, :, :keys]
+
+    near = run(keys, False)
+    ref = Attention(q, k, v, lengths).backward(dout)
+    for pad, longer in ((1000, False), (1000, True), (129, True)):
+        far = run(pad, longer)
+        # one tile of keys: dQ is the same sum of the same products
+        one_tile = [i for i, n in enumerate(lens) if n <= 64]
+        assert torch.equal(far[0][one_tile], near[0][one_tile])
+        for name, x, y in zip(("dq", "dk", "dv"), far, near):
+            want, bound = ref[name]
+            assert_within(x, want, bound, name)
+            # others are summed in another order in 32 bits: a result next to a
+            # border between two of its type's numbers falls on either side
+            off = (x.double() - y.double()).norm() / y.double().norm().clamp_min(1e-30)
+            assert off < U[dtype] / 4, (name, off)
