@@ -4,8 +4,10 @@
 //   dw = sum over rows of dy h,  db = sum over rows of dy
 // Both directions are bound by memory: x (and dy) are read once and held in
 // registers, in fp32 statistics over the deviations from the mean (a second
-// pass over registers, not a difference of large sums; divided by n, so that a
-// constant row has that very mean).  LANES threads share a
+// pass over registers, not a difference of large sums).  The sum of x rounds, so
+// that mean misses by an amount that goes with |mean| and not with the row's
+// spread; the deviations' own sum, taken beside their squares', puts it right: a
+// constant row has that very mean and a variance of zero.  LANES threads share a
 // row (16, a wave, or a workgroup), each with CH chunks of 16 bytes; they walk
 // rows with the weights in registers.  Rows too wide for that are read again
 // from the caches.  dw and db are summed per thread over the rows of its
@@ -44,6 +46,40 @@ __device__ __forceinline__ float row_sum(float v, float* slot) {
     }
   }
   return v;
+}
+
+// The same for two sums at once.
+template <int LANES>
+__device__ __forceinline__ void row_sums(float& v, float& u, float* slot_v, float* slot_u) {
+  constexpr int W = LANES < 64 ? LANES : 64;
+#pragma unroll
+  for (int x = W / 2; x > 0; x >>= 1) {
+    v += __shfl_xor(v, x);
+    u += __shfl_xor(u, x);
+  }
+  if constexpr (LANES > 64) {
+    if ((threadIdx.x & 63) == 0) {
+      slot_v[threadIdx.x >> 6] = v;
+      slot_u[threadIdx.x >> 6] = u;
+    }
+    __syncthreads();
+    v = 0.0f;
+    u = 0.0f;
+#pragma unroll
+    for (int w = 0; w < LANES / 64; ++w) {
+      v += slot_v[w];
+      u += slot_u[w];
+    }
+  }
+}
+
+// mean, and deviations d from it with their sum and their squares' sum: how far
+// the deviations' mean is from zero.  Returns 1 / sqrt(var + eps).
+__device__ __forceinline__ float put_right(float sum, float squares, float n, float eps, float& mean, float& off) {
+  off = sum / n;
+  mean += off;
+  const float var = fmaf(-off, off, squares / n);
+  return 1.0f / sqrtf((var < 0.0f ? 0.0f : var) + eps);
 }
 
 // Value i of the weights, which are in x's type or fp32.
@@ -136,7 +172,7 @@ __global__ __launch_bounds__(kThreads) void ln_fwd_kernel(LayerNormArgs a) {
   using E = typename Elem<T>::type;
   constexpr int EC = Elem<T>::kChunk;
   constexpr int RPB = kThreads / LANES;  // rows of a workgroup at a time
-  __shared__ float sums[4][kThreads / 64];
+  __shared__ float sums[6][kThreads / 64];
   const int lane = threadIdx.x % LANES;
   const int64_t step = static_cast<int64_t>(gridDim.x) * RPB;
   float w[CH][EC], bias[CH][EC];
@@ -174,18 +210,22 @@ __global__ __launch_bounds__(kThreads) void ln_fwd_kernel(LayerNormArgs a) {
     if (k + 1 < rounds) {
       fetch(row + step);
     }
-    const float mean = row_sum<LANES>(s, sums[flip]) / n;
+    float mean = row_sum<LANES>(s, sums[flip]) / n;
     s = 0.0f;
+    float s1 = 0.0f;
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
 #pragma unroll
       for (int i = 0; i < EC; ++i) {
         x[c][i] = (c * LANES + lane) * EC + i < a.n ? x[c][i] - mean : 0.0f;
+        s1 += x[c][i];
         s = fmaf(x[c][i], x[c][i], s);
       }
     }
-    const float rstd = 1.0f / sqrtf(row_sum<LANES>(s, sums[flip + 1]) / n + a.eps);
-    flip ^= 2;
+    row_sums<LANES>(s, s1, sums[flip + 1], sums[flip + 2]);
+    float off;
+    const float rstd = put_right(s1, s, n, a.eps, mean, off);
+    flip ^= 3;
     if (row < a.rows) {
       E* yr = static_cast<E*>(a.y) + row * a.sy;
 #pragma unroll
@@ -193,7 +233,7 @@ __global__ __launch_bounds__(kThreads) void ln_fwd_kernel(LayerNormArgs a) {
         float y[EC];
 #pragma unroll
         for (int i = 0; i < EC; ++i) {
-          y[i] = fmaf(x[c][i] * rstd, w[c][i], bias[c][i]);
+          y[i] = fmaf((x[c][i] - off) * rstd, w[c][i], bias[c][i]);
         }
         store_chunk<T, VEC>(yr, c * LANES + lane, a.n, y);
       }
@@ -210,7 +250,7 @@ template <typename T, bool VEC>
 __global__ __launch_bounds__(kThreads) void ln_fwd_wide_kernel(LayerNormArgs a) {
   using E = typename Elem<T>::type;
   constexpr int EC = Elem<T>::kChunk;
-  __shared__ float sums[2][kThreads / 64];
+  __shared__ float sums[3][kThreads / 64];
   const float n = static_cast<float>(a.n);
   const int chunks = (a.n + EC - 1) / EC;
   for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
@@ -225,17 +265,21 @@ __global__ __launch_bounds__(kThreads) void ln_fwd_wide_kernel(LayerNormArgs a) 
       }
     }
     __syncthreads();
-    const float mean = row_sum<kThreads>(s, sums[0]) / n;
+    const float first = row_sum<kThreads>(s, sums[0]) / n;
     s = 0.0f;
+    float s1 = 0.0f;
     for (int c = threadIdx.x; c < chunks; c += kThreads) {
       const u32x4 v = load_chunk<T, VEC>(xr, c, a.n);
 #pragma unroll
       for (int i = 0; i < EC; ++i) {
-        const float d = c * EC + i < a.n ? chunk_value<T>(v, i) - mean : 0.0f;
+        const float d = c * EC + i < a.n ? chunk_value<T>(v, i) - first : 0.0f;
+        s1 += d;
         s = fmaf(d, d, s);
       }
     }
-    const float rstd = 1.0f / sqrtf(row_sum<kThreads>(s, sums[1]) / n + a.eps);
+    row_sums<kThreads>(s, s1, sums[1], sums[2]);
+    float mean = first, off;
+    const float rstd = put_right(s1, s, n, a.eps, mean, off);
     for (int c = threadIdx.x; c < chunks; c += kThreads) {
       const u32x4 v = load_chunk<T, VEC>(xr, c, a.n);
       float y[EC];
@@ -244,7 +288,7 @@ __global__ __launch_bounds__(kThreads) void ln_fwd_wide_kernel(LayerNormArgs a) 
         const int at = c * EC + i;
         const float w = a.w != nullptr && at < a.n ? weight_at<T>(a.w, a.wide, at) : 1.0f;
         const float b = a.b != nullptr && at < a.n ? weight_at<T>(a.b, a.wide, at) : 0.0f;
-        y[i] = fmaf((chunk_value<T>(v, i) - mean) * rstd, w, b);
+        y[i] = fmaf((chunk_value<T>(v, i) - first - off) * rstd, w, b);
       }
       store_chunk<T, VEC>(yr, c, a.n, y);
     }
