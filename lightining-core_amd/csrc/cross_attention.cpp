@@ -102,8 +102,8 @@ Status checkConfig(const lcCrossAttentionConfig* c) {
   if (!validDtype(c->dtype)) {
     return fail(Status::kInvalidValue, "cross attention: dtype must be f32, bf16 or f16");
   }
-  if (!std::isfinite(c->scale)) {
-    return fail(Status::kInvalidValue, "cross attention: scale is not finite");
+  if (!std::isfinite(c->scale * kLog2e)) {
+    return fail(Status::kInvalidValue, "cross attention: scale is not finite in exp2 units");
   }
   if (c->head_dim > kern::kXAttnMaxDim) {
     return fail(Status::kNotSupported, "cross attention: head_dim <= 128");
@@ -126,7 +126,7 @@ void fillArgs(const lcCrossAttentionConfig& c, kern::XAttnArgs* a) {
   a->kv_len = static_cast<int>(c.kv_len);
   a->d = static_cast<int>(c.head_dim);
   a->scale = c.scale != 0.0f ? c.scale : 1.0f / std::sqrt(static_cast<float>(c.head_dim));
-  a->c = std::fabs(a->scale) * 1.4426950408889634f;
+  a->c = std::fabs(a->scale) * kLog2e;
   a->negate = a->scale < 0.0f ? 1 : 0;
 }
 

@@ -9,6 +9,8 @@
 
 namespace lchip {
 
+constexpr float kLog2e = 1.4426950408889634f;  // the softmax runs on exp2
+
 // The scope of such a call: the library's device is current inside it and the
 // caller's is again afterwards.
 class DeviceCall {

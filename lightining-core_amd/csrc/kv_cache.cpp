@@ -134,8 +134,8 @@ Status checkAttn(const lcKvCache* cache, const lcKvAttentionConfig* cfg, AttnPla
   if (!validDtype(cfg->dtype)) {
     return fail(Status::kInvalidValue, "kv cache: dtype must be f32, bf16 or f16");
   }
-  if (!std::isfinite(cfg->scale)) {
-    return fail(Status::kInvalidValue, "kv cache: scale is not finite");
+  if (!std::isfinite(cfg->scale * kLog2e)) {
+    return fail(Status::kInvalidValue, "kv cache: scale is not finite in exp2 units");
   }
   const std::size_t group = cfg->heads / cache->kv_heads;
   if (cfg->batch > kMost || cfg->heads > kMost || cfg->q_len > kMost || cfg->batch * cache->kv_heads > kMost ||
@@ -206,7 +206,7 @@ Status attention(const lcKvCache* cache, const lcKvAttentionConfig* cfg, const l
   a.d = static_cast<int>(c.head_dim);
   a.pages = static_cast<int>(c.pages);
   const float scale = cfg->scale != 0.0f ? cfg->scale : 1.0f / std::sqrt(static_cast<float>(c.head_dim));
-  a.c = scale * 1.4426950408889634f;
+  a.c = scale * kLog2e;
   a.aligned = q_aligned ? 1 : 0;
   a.splits = plan.splits;
   a.part = static_cast<float*>(workspace);

@@ -35,6 +35,7 @@ __all__ = ["cross_attention", "cross_attention_backward", "layer_norm", "layer_n
 KV_PAGE_TOKENS = 64
 
 _byref = ctypes.byref
+_MOST_SCALE = 2.3e38  # times log2(e) it is still an fp32 number
 
 
 def _is_torch(x) -> bool:
@@ -322,10 +323,11 @@ def _scale(scale):
     """The library's convention: 0 for 1 / sqrt(head_dim)."""
     if scale is None:
         return 0.0
-    scale = float(scale)
-    if scale == 0.0 or scale != scale or scale in (float("inf"), float("-inf")):
-        raise ValueError("scale must be a finite number other than zero")
-    return scale
+    # As fp32, which is what the library gets: 1e-46 would reach it as 0.
+    got = ctypes.c_float(scale).value
+    if got == 0.0 or not abs(got) < _MOST_SCALE:
+        raise ValueError(f"scale must be a number other than zero that fp32 holds, below 2.3e38: {scale}")
+    return got
 
 
 def _lengths(call, x, batch):
