@@ -9,9 +9,10 @@ numpy arrays (results are numpy arrays; the call returns when they are there).
 Import torch before the library's first call: torch brings a HIP runtime of its
 own, and a process in which the library has already started another one has no
 device for torch.  The results carry no autograd history: a training step calls
-the backward functions itself.  Shapes, types and layouts that a call does not take raise
-ValueError; a status of the library raises RuntimeError, as everywhere in this
-package.
+the backward functions itself, and a tensor that requires a gradient is refused
+unless the call is made under torch.no_grad().  Shapes, types and layouts that a
+call does not take raise ValueError; a status of the library raises RuntimeError,
+as everywhere in this package.
 """
 from __future__ import annotations
 
@@ -59,6 +60,7 @@ class _Torch:
         self._types = {v: k for k, v in self._dtypes.items()}
         self._tensor = torch.Tensor
         self._empty = torch.empty
+        self._tracking = torch.is_grad_enabled
         self._int32, self._float32 = torch.int32, torch.float32
         # The stream's handle without a Stream object around it (2 us a call less).
         raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
@@ -74,6 +76,9 @@ class _Torch:
             raise ValueError(f"{name} must be a torch tensor, as the other arguments are")
         if not x.is_cuda or x.get_device() != self.index:
             raise ValueError(f"{name} is on {x.device}, the other tensors on {self.device}")
+        if x.requires_grad and self._tracking():
+            raise ValueError(f"{name} requires a gradient that this call would not record: call it under "
+                             "torch.no_grad() or with detached tensors, and the backward functions for gradients")
         return x
 
     def dtype(self, x, name):
@@ -392,7 +397,8 @@ def cross_attention(q, k, v, kv_lengths=None, *, scale=None, return_lse=False, o
     kv_lengths int32 [batch] (None: kv_len everywhere), held to [0, kv_len].
     scale defaults to 1 / sqrt(head_dim).  A row without keys gives zeros.
     Returns out like q, with return_lse also the log of each row's sum of
-    exponentials, float32 [batch, heads, q_len] (-inf without keys).
+    exponentials, float32 [batch, heads, q_len] (-inf without keys).  No autograd
+    history: cross_attention_backward gives the gradients.
     """
     call = _call_of(q)
     q, k, v, (cfg, nbytes, _) = _xattn_inputs(call, q, k, v, scale)
@@ -465,7 +471,8 @@ def layer_norm(x, weight=None, bias=None, *, eps=1e-5, return_stats=False):
     x [..., n], float32, bfloat16 or float16, its leading dimensions rows of one
     stride; weight, bias [n] of x's type or float32 (both the same), or None.
     Returns y (contiguous, like x), with return_stats also mean and
-    rstd = 1 / sqrt(var + eps), float32 [...].
+    rstd = 1 / sqrt(var + eps), float32 [...].  No autograd history:
+    layer_norm_backward gives the gradients.
     """
     call = _call_of(x)
     x = call.take(x, "x")
@@ -594,7 +601,7 @@ def kv_cache_attention(q, k_pages, v_pages, k_scales, v_scales, block_table, kv_
     kv_lengths int32 [batch] (None: every token of the table's pages).  Made for
     few query rows, such as a decode step's.  A table entry outside the pool is
     not read; rows that would need it come out as NaN.  Returns as
-    cross_attention does.
+    cross_attention does; there is no gradient.
     """
     call = _call_of(q)
     q = call.take(q, "q")
