@@ -497,10 +497,12 @@ def layer_norm(x, weight=None, bias=None, *, eps=1e-5, return_stats=False):
     return got if return_stats else got[0]
 
 
-def layer_norm_backward(dy, x, weight, mean, rstd):
+def layer_norm_backward(dy, x, weight, mean, rstd, *, bias=None):
     """Gradients (dx, dweight, dbias) of layer_norm for the gradient dy of its
     result.  mean and rstd are what layer_norm(..., return_stats=True) returned.
-    dweight and dbias are in weight's type; both None when weight is.
+    dweight and dbias are in weight's type; with weight None, dweight is None and
+    so is dbias, unless the bias that layer_norm took alone is given (its values
+    do not matter, dbias is of its type).
     """
     call = _call_of(x)
     x, dy = call.take(x, "x"), call.take(dy, "dy")
@@ -513,6 +515,11 @@ def layer_norm_backward(dy, x, weight, mean, rstd):
     wd = dtype
     if weight is not None:
         weight, wd = _vector(call, weight, n, dtype, "weight")
+    if bias is not None:
+        bias, bd = _vector(call, bias, n, dtype, "bias")
+        if weight is not None and bd != wd:
+            raise ValueError("weight and bias must have one type")
+        wd = bd
     mean, rstd = call.take(mean, "mean"), call.take(rstd, "rstd")
     for s, name in ((mean, "mean"), (rstd, "rstd")):
         _same(s, x.shape[:-1], name)
@@ -523,6 +530,8 @@ def layer_norm_backward(dy, x, weight, mean, rstd):
     dw = db = None
     if weight is not None:
         dw, db = call.empty_contiguous(weight), call.empty_contiguous(weight)
+    elif bias is not None:
+        db = call.empty_contiguous(bias)
     ws = call.workspace(nbytes)
     call.run("lcLayerNormBackward", "ipipippppipppii",
              (cfg.at, dy, dy_stride, x, stride, weight, mean, rstd, dx, n, dw, db, ws, nbytes, call.stream), "")
