@@ -36,6 +36,7 @@ __all__ = ["cross_attention", "cross_attention_backward", "layer_norm", "layer_n
 KV_PAGE_TOKENS = 64
 
 _byref = ctypes.byref
+_INT32_MOST = 2**31 - 1
 _MOST_SCALE = 2.3e38  # times log2(e) it is still an fp32 number
 
 
@@ -232,6 +233,11 @@ class _Numpy:
         x = np.asarray(x)
         if x.dtype.kind not in "iu":
             raise ValueError(f"{name} must hold integers")
+        if x.dtype.itemsize > 2 and x.dtype != np.int32:
+            # Numbers past 32 bits stay past every length and every pool.
+            x = np.minimum(x, _INT32_MOST)
+            if x.dtype.kind == "i":
+                x = np.maximum(x, -_INT32_MOST)
         return np.ascontiguousarray(x, dtype=np.int32)
 
     def strides(self, x):

@@ -2,6 +2,7 @@
 (CPU only)."""
 import ctypes
 
+import numpy as np
 import pytest
 
 from lightning_core import _decoder
@@ -29,3 +30,19 @@ def test_scales_reach_the_library_as_they_are():
     for scale in (1.0, -2.5, 0.1, 1e-45, 2.2e38):
         assert _decoder._scale(scale) == ctypes.c_float(scale).value != 0
         assert _size(_decoder._scale(scale))[0] == 0
+
+
+@pytest.mark.parametrize("kind", ["i1", "u1", "i2", "u2", "i4", "u4", "i8", "u8"])
+def test_integers_of_numpy_arrays_keep_their_order(kind):
+    """What passes 32 bits is held to them, not wrapped: a length of 2^32 + 1 is not 1."""
+    info = np.iinfo(kind)
+    values = [v for v in (0, 1, 5, 100, 2**31 - 1, 2**31, 2**32, 2**32 + 1, 2**63 - 1, 2**64 - 1, -1, -7, -2**31,
+                          -2**32 + 3, -2**63) if info.min <= v <= info.max]
+    got = _decoder._Numpy.ints(None, np.array(values, dtype=kind), "kv_lengths")
+    assert got.dtype == np.int32
+    for v, g in zip(values, got.tolist()):
+        assert g == max(min(v, 2**31 - 1), -2**31) or (v < -2**30 and g < -2**30)
+    assert _decoder._Numpy.ints(None, [3, 4], "kv_lengths").tolist() == [3, 4]
+    for bad in ([1.5], [True], ["a"]):
+        with pytest.raises(ValueError, match="integers"):
+            _decoder._Numpy.ints(None, np.array(bad), "kv_lengths")
