@@ -133,6 +133,10 @@ class _Torch:
     def is_contiguous(x):
         return x.is_contiguous()
 
+    @staticmethod
+    def writable(*tensors):
+        """Tensors have no such mark."""
+
     def workspace(self, nbytes):
         """Scratch of a call, held by the caller until the call is queued: the
         allocator hands it out again only to work queued behind it on the same
@@ -279,6 +283,12 @@ class _Numpy:
     def is_contiguous(self, x):
         return x.flags.c_contiguous
 
+    @staticmethod
+    def writable(*arrays):
+        for x, name in arrays:
+            if not x.flags.writeable:
+                raise ValueError(f"{name} is written and read-only")
+
     def workspace(self, nbytes):
         return np.empty(nbytes, np.uint8) if nbytes else None
 
@@ -358,6 +368,7 @@ def _out(call, out, like, name):
     if isinstance(call, _Numpy):
         if not isinstance(out, np.ndarray) or not out.flags.c_contiguous:
             raise ValueError(f"{name} must be a contiguous array")
+        call.writable((out, name))
     else:
         out = call.take(out, name)
     if out.dtype != like.dtype:
@@ -590,6 +601,7 @@ def kv_cache_store(k, v, block_table, kv_lengths, k_pages, v_pages, k_scales, v_
     c, pool = _cache(call, k_pages, v_pages, k_scales, v_scales)
     if (h, d) != (c.kv_heads, c.head_dim):
         raise ValueError("k and the cache must agree in kv_heads and head_dim")
+    call.writable(*zip(pool, ("k_pages", "v_pages", "k_scales", "v_scales")))
     lengths = _lengths(call, kv_lengths, b)
     t, stride = _table(call, block_table, b)
     call.run("lcKvCacheStore", "iiiittpiipi",
