@@ -69,9 +69,26 @@ Status takeTensor(const char* op, const char* name, const lcDeviceTensor* t, std
     return fail(Status::kNotSupported, who + " has a stride too large");
   }
   if (written) {
-    const std::int64_t dd = static_cast<std::int64_t>(d);
-    if ((batch > 1 && out->sb < dd) || (heads > 1 && out->sh < dd) || (rows > 1 && out->ss < dd)) {
-      return fail(Status::kInvalidValue, who + " is written and has overlapping rows");
+    // From the smallest stride up, each step must pass all that lies inside it
+    // (the padding behind a block's last row may hold the next block's rows).
+    struct Dim {
+      std::int64_t stride;
+      std::size_t n;
+    } dims[] = {{out->sb, batch}, {out->sh, heads}, {out->ss, rows}};
+    std::sort(dims, dims + 3, [](const Dim& x, const Dim& y) { return x.stride < y.stride; });
+    std::int64_t extent = static_cast<std::int64_t>(d);
+    for (const Dim& x : dims) {
+      if (x.n == 1) {
+        continue;
+      }
+      if (x.stride < extent) {
+        return fail(Status::kInvalidValue, who + " is written and has overlapping rows");
+      }
+      // No product of a stride that a real tensor can have overflows.
+      if (x.stride > (std::int64_t{1} << 62) / static_cast<std::int64_t>(x.n)) {
+        return fail(Status::kNotSupported, who + " has a stride too large");
+      }
+      extent += x.stride * static_cast<std::int64_t>(x.n - 1);
     }
   }
   const std::int64_t ec = static_cast<std::int64_t>(16 / bytes);

@@ -41,8 +41,8 @@ inline std::size_t bytesOf(lcDataType t) { return t == LC_DTYPE_F32 ? 4 : 2; }
 // A [batch, heads, rows, d] tensor as the kernels take it.  kInvalidValue for a
 // null base of a tensor with values, a base off its elements' alignment or a
 // negative stride; kNotSupported for a row stride whose tile of 128 rows passes
-// 2^31 bytes (the kernels' offsets within a tile).  `written`: also kInvalidValue where two of its rows overlap by a
-// stride smaller than d.  Clears *aligned unless 16-byte accesses suit it.
+// 2^31 bytes (the kernels' offsets within a tile).  `written`: also kInvalidValue where two of its rows share memory.
+// Clears *aligned unless 16-byte accesses suit it.
 Status takeTensor(const char* op, const char* name, const lcDeviceTensor* t, std::size_t batch, std::size_t heads,
                   std::size_t rows, std::size_t d, lcDataType type, bool written, kern::XTensor* out, bool* aligned);
 

@@ -413,6 +413,7 @@ def cross_attention(q, k, v, kv_lengths=None, *, scale=None, return_lse=False, o
     float32, bfloat16 or float16; any strides with a contiguous last dimension.
     kv_lengths int32 [batch] (None: kv_len everywhere), held to [0, kv_len].
     scale defaults to 1 / sqrt(head_dim).  A row without keys gives zeros.
+    out, if given, receives the result; it must not share memory with k or v.
     Returns out like q, with return_lse also the log of each row's sum of
     exponentials, float32 [batch, heads, q_len] (-inf without keys).  No autograd
     history: cross_attention_backward gives the gradients.
@@ -421,6 +422,8 @@ def cross_attention(q, k, v, kv_lengths=None, *, scale=None, return_lse=False, o
     q, k, v, (cfg, nbytes, _) = _xattn_inputs(call, q, k, v, scale)
     lengths = _lengths(call, kv_lengths, q.shape[0])
     out = _out(call, out, q, "out")
+    if out is k or out is v:
+        raise ValueError("out must not be k or v")
     lse = call.empty(q, q.shape[:3], N.LC_DTYPE_F32) if return_lse else None
     ws = call.workspace(nbytes)
     call.run("lcCrossAttentionForward", "itttptppii", (cfg.at, q, k, v, lengths, out, lse, ws, nbytes, call.stream),

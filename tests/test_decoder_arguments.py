@@ -46,3 +46,31 @@ def test_integers_of_numpy_arrays_keep_their_order(kind):
     for bad in ([1.5], [True], ["a"]):
         with pytest.raises(ValueError, match="integers"):
             _decoder._Numpy.ints(None, np.array(bad), "kv_lengths")
+
+
+@pytest.mark.parametrize("strides,shape,fits", [
+    ((384, 192, 64), (2, 2, 3), True),      # batch, heads, rows in order
+    ((384, 64, 128), (2, 2, 3), True),      # rows that hold both heads
+    ((64, 768, 128), (2, 2, 3), True),      # the batch innermost
+    ((400, 196, 65), (2, 2, 3), True),      # padding behind rows and heads
+    ((64, 64, 128), (2, 2, 3), False),      # two batch rows in the heads' place
+    ((192, 192, 64), (2, 2, 3), False),     # batch and heads one apart
+    ((128, 192, 64), (2, 2, 3), False),     # a head reaches into the next
+    ((384, 192, 63), (2, 2, 3), False),
+    ((0, 0, 0), (1, 1, 1), True),           # nothing to step over
+    ((0, 64, 128), (1, 2, 3), True),
+    ((0, 64, 128), (2, 2, 3), False),
+])
+def test_written_tensors_do_not_overlap_themselves(strides, shape, fits):
+    """Checked before the device is opened: a tensor that fits gets as far as the
+    next one, which has no base."""
+    lib = N.load()
+    b, h, s = shape
+    cfg = N.CrossAttentionConfig(b, h, h, s, s, 64, N.LC_DTYPE_F16, 0.0)
+    r = ctypes.byref
+    ok, none = N.DeviceTensor(256, h * s * 64, s * 64, 64), N.DeviceTensor(None, h * s * 64, s * 64, 64)
+    dq = N.DeviceTensor(256, *strides)
+    assert lib.lcCrossAttentionBackward(r(cfg), r(ok), r(ok), r(ok), r(ok), r(ok), 256, None, r(dq), r(none), r(ok),
+                                        None, 0, None) == N.LC_INVALID_VALUE
+    message = lib.lcGetLastErrorMessage().decode()
+    assert ("dk has values and a null base" in message) if fits else ("dq is written and has overlapping" in message)
