@@ -580,8 +580,11 @@ typedef struct lcKvCache {
 /* Writes the first kv_lengths[b] (NULL: kv_len) tokens of k, v
  * [batch, kv_heads, kv_len, head_dim] to row b's pages, from their start: scale
  * = max(amax / 448, 2^-126) over a page of one head, code = e4m3(x / scale) to
- * the nearest, ties to even; the rest of a last page becomes zeros.  A page
- * outside the pool is not written; pages that no row names stay as they are.
+ * the nearest, ties to even; the rest of a last page becomes zeros.  A NaN has
+ * no part in amax and keeps a NaN code: what attends to its token (keys), or its
+ * column (values), is NaN, the rest of its page is as without it.  An infinity
+ * makes its page's scale of that head infinite, and attention over the page NaN.
+ * A page outside the pool is not written; pages that no row names stay as they are.
  * Rows that name one page must bring the same tokens for it. */
 lcError_t lcKvCacheStore(const lcKvCache* cache, size_t batch, size_t kv_len, lcDataType dtype,
                          const lcDeviceTensor* k, const lcDeviceTensor* v, const int32_t* block_table,

@@ -59,7 +59,8 @@ __device__ __forceinline__ uint32_t codes4(float a, float b, float c, float d) {
 // One workgroup writes a page's head: thread (token quad, 8 columns) holds four
 // tokens of K and of V, so that a page is read once, its scale is known before
 // any code is made, and V's codes come out as dwords of four tokens.  Tokens
-// past the row's length are zero codes.
+// past the row's length are zero codes.  fmaxf leaves a NaN out of the maximum:
+// one bad value does not cost its page the other 64 d - 1.
 template <typename T, bool VEC>
 __global__ __launch_bounds__(256) void kv_store_kernel(KvStoreArgs a) {
   using E = typename Elem<T>::type;

@@ -592,7 +592,8 @@ def kv_cache_store(k, v, block_table, kv_lengths, k_pages, v_pages, k_scales, v_
     float8_e4m3fn), k_scales and v_scales float32 [pages, kv_heads].  Row b's
     first kv_lengths[b] tokens go to the pages block_table[b] from their start,
     each page and head with a scale of max(amax / 448, 2^-126); the rest of its
-    last page becomes zeros and no other page changes.  Pages outside the pool
+    last page becomes zeros and no other page changes.  A NaN has no part in amax
+    and stays one; an infinity makes its whole page NaN.  Pages outside the pool
     are not written.  Rows that name one page must bring the same tokens for it.
     """
     call = _call_of(k)
