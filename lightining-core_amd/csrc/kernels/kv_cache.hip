@@ -401,9 +401,11 @@ __global__ __launch_bounds__(256, 2) void kv_attn_kernel(KvAttnArgs a) {
       terms<NP>(v, pt[u]);
     }
     // Codes behind the last token may be anything: a NaN there must not meet its
-    // probability of zero.  (Every page is masked, 4 instructions a load: with a
-    // branch around it the compiler gave registers of V to the probabilities'
-    // terms while V was still needed.)
+    // probability of zero.  (Every page is masked, 4 instructions a load: behind a
+    // branch around it the compiler, clang 22 of ROCm 7.2.0, wrote a term of the
+    // probabilities into v46, which still held codes of V that it widened 50
+    // instructions later.  tests/test_asm_kv_values.py looks for that in the
+    // compiled kernels.)
     u32x4 keep;
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
