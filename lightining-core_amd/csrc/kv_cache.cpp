@@ -146,12 +146,16 @@ Status checkAttn(const lcKvCache* cache, const lcKvAttentionConfig* cfg, AttnPla
   plan->width = static_cast<std::size_t>(kern::kXAttnWidth(static_cast<int>(cache->head_dim)));
   const std::size_t blocks = cfg->batch * cache->kv_heads * ((group * cfg->q_len + kRows - 1) / kRows);
   // A split has at least a page for each of its four waves.  Rows differ in
-  // length and the host does not know by how much: long tables are split twice as
-  // often as would fill the chip, so that short rows' workgroups make room (32
-  // rows of 64 to 128 pages: 85.5 -> 80.9 us; four times as often 85.0).
+  // length and the host does not know by how much: tables that are split to fill
+  // the chip are split twice as often when they are long, so that short rows'
+  // workgroups make room.  us, once -> twice, 32 rows x 8 heads of 128 pages: 64
+  // to 128 in use 76 -> 71, one row of 128 among rows of 16 63 -> 42, all in use
+  // 86 -> 88.  Where the blocks fill the chip unsplit a second share only adds a
+  // join and its workspace: 64 x 8 heads of 64 pages 83 -> 87, half in use 69 ->
+  // 71; 64 rows of 16 x 32 heads 183 -> 307, of 512 x 4 x 32 94 -> 122.
   const std::size_t quads = (cfg->table_width + 3) / 4;
   const int splits = splitCount(blocks, quads, kSlots, 1.0, 3.0);
-  plan->splits = quads >= 8u * splits ? 2 * splits : splits;
+  plan->splits = splits > 1 && quads >= 8u * splits ? 2 * splits : splits;
   return Status::kSuccess;
 }
 
