@@ -10,6 +10,7 @@ namespace {
 
 constexpr const char* kOp = "cross attention";
 constexpr std::size_t kMostRows = std::size_t{1} << 30;
+constexpr std::size_t kMostProblems = std::size_t{1} << 24;
 // Workgroups that run at once on 256 CUs: two a CU, of the few-row forward one.
 constexpr std::size_t kSlots = 512;
 constexpr std::size_t kFewSlots = 256;
@@ -108,10 +109,11 @@ Status checkConfig(const lcCrossAttentionConfig* c) {
   if (c->head_dim > kern::kXAttnMaxDim) {
     return fail(Status::kNotSupported, "cross attention: head_dim <= 128");
   }
-  // Row indices and grids are 32-bit.
+  // Row indices are 32-bit, and a launch has less than 2^32 threads a dimension:
+  // 256 a problem.
   const std::size_t most = kMostRows;
   if (c->batch > most || c->heads > most || c->q_len > most || c->kv_len > most ||
-      c->batch * c->kv_heads > most || (c->heads / c->kv_heads) * c->q_len > most / 512 ||
+      c->batch * c->kv_heads >= kMostProblems || (c->heads / c->kv_heads) * c->q_len > most / 512 ||
       c->kv_len > most / 512) {
     return fail(Status::kNotSupported, "cross attention: shape too large");
   }

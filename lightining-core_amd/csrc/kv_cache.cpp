@@ -10,6 +10,7 @@ namespace {
 
 constexpr const char* kOp = "kv cache";
 constexpr std::size_t kMost = std::size_t{1} << 30;
+constexpr std::size_t kMostProblems = std::size_t{1} << 24;
 // Workgroups of four waves that run at once.
 constexpr std::size_t kSlots = 512;
 constexpr std::size_t kRows = 16;  // query rows of a workgroup
@@ -138,7 +139,8 @@ Status checkAttn(const lcKvCache* cache, const lcKvAttentionConfig* cfg, AttnPla
     return fail(Status::kInvalidValue, "kv cache: scale is not finite in exp2 units");
   }
   const std::size_t group = cfg->heads / cache->kv_heads;
-  if (cfg->batch > kMost || cfg->heads > kMost || cfg->q_len > kMost || cfg->batch * cache->kv_heads > kMost ||
+  // 256 threads a problem, and a launch has less than 2^32 a dimension.
+  if (cfg->batch > kMost || cfg->heads > kMost || cfg->q_len > kMost || cfg->batch * cache->kv_heads >= kMostProblems ||
       group * cfg->q_len > kRows * 65535 || cfg->table_width > kMost / kern::kKvPage) {
     return fail(Status::kNotSupported, "kv cache: shape too large");
   }

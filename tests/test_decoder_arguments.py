@@ -74,3 +74,22 @@ def test_written_tensors_do_not_overlap_themselves(strides, shape, fits):
                                         None, 0, None) == N.LC_INVALID_VALUE
     message = lib.lcGetLastErrorMessage().decode()
     assert ("dk has values and a null base" in message) if fits else ("dq is written and has overlapping" in message)
+
+
+def test_problems_past_a_launch_are_not_supported():
+    """256 threads a (batch row, key/value head) pair, less than 2^32 in a launch."""
+    lib = N.load()
+
+    def attention(b, heads):
+        cfg = N.CrossAttentionConfig(b, heads, heads, 1, 1, 16, N.LC_DTYPE_F16, 0.0)
+        return lib.lcCrossAttentionWorkspaceSize(ctypes.byref(cfg), 0, ctypes.byref(ctypes.c_size_t()))
+
+    def cached(b, heads):
+        pool = N.KvCache(256, 256, 256, 256, 4, heads, 16)
+        cfg = N.KvAttentionConfig(b, heads, 1, 1, N.LC_DTYPE_F16, 0.0)
+        return lib.lcKvCacheAttentionWorkspaceSize(ctypes.byref(pool), ctypes.byref(cfg),
+                                                   ctypes.byref(ctypes.c_size_t()))
+
+    for call in (attention, cached):
+        assert call((1 << 24) - 1, 1) == 0 and call((1 << 23) - 1, 2) == 0
+        assert call(1 << 24, 1) == N.LC_NOT_SUPPORTED and call(1 << 22, 4) == N.LC_NOT_SUPPORTED
