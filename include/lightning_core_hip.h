@@ -507,7 +507,10 @@ typedef struct lcDeviceTensor {
  * past a row's length are not read.  head_dim <= 128 (else LC_NOT_SUPPORTED);
  * q_len, kv_len and batch may be 0; scale 0 means 1 / sqrt(head_dim).
  * Sums, the softmax and products accumulate in fp32; with 16-bit types the
- * probabilities are rounded to that type for the second product. */
+ * probabilities are rounded to that type for the second product, where fp32 would
+ * halve its rate or more (fp16: the largest one of a row lies between 2^7 and
+ * 2^15, so that a tail of small ones keeps its bits).  That is half a step of the
+ * type a probability, beside the half step of the result. */
 typedef struct lcCrossAttentionConfig {
   size_t batch;
   size_t heads;
@@ -527,7 +530,13 @@ lcError_t lcCrossAttentionForward(const lcCrossAttentionConfig* cfg, const lcDev
 /* Gradients of the forward with the same cfg and kv_lengths; out and lse are
  * its results.  dq like q; dk, dv like k, v (summed over the query heads that
  * share a head; zero past a row's length).  Every gradient is written by one
- * workgroup or summed in a fixed order: equal calls give equal bits. */
+ * workgroup or summed in a fixed order: equal calls give equal bits.  With 16-bit
+ * types the second products take P (for dv) and dS = P o (dP - delta) (for dq and
+ * dk) rounded to that type; fp16 holds both at powers of two, dS at one for each
+ * query row and key, so that results inside fp16 keep its precision whatever the
+ * size of dout and v and the number of keys (P below 2^-29 counts less exactly).
+ * delta is the sum of P dP over a row's keys up to 128 of them, and of dout out,
+ * with `out` as it was rounded, beyond. */
 lcError_t lcCrossAttentionBackward(const lcCrossAttentionConfig* cfg, const lcDeviceTensor* dout,
                                    const lcDeviceTensor* q, const lcDeviceTensor* k, const lcDeviceTensor* v,
                                    const lcDeviceTensor* out, const float* lse, const int32_t* kv_lengths,

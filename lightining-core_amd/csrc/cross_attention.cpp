@@ -11,7 +11,9 @@ namespace {
 constexpr const char* kOp = "cross attention";
 constexpr std::size_t kMostRows = std::size_t{1} << 30;
 constexpr std::size_t kMostProblems = std::size_t{1} << 24;
-// Workgroups that run at once on 256 CUs: two a CU, of the few-row forward one.
+// Workgroups that the shares are cut for, on 256 CUs: two a CU, of the few-row
+// forward one.  Where a CU holds only one of the former (fp32 rows wider than 64,
+// rows that no vector load suits), a round of workgroups takes two rounds' time.
 constexpr std::size_t kSlots = 512;
 constexpr std::size_t kFewSlots = 256;
 // The forward's waves share the keys of 32 rows, instead of taking 32 rows each,

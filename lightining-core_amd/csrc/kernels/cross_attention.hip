@@ -780,7 +780,7 @@ __global__ __launch_bounds__(256) void xattn_join_kernel(XAttnArgs a) {
 // [2^7, 2^8), and e falls when a later one would pass 2^15.  What the largest
 // value so far leaves normal reaches down to 2^-21 of it.  (A scale from dO
 // alone lets dS overflow for large V: two keys of 20000 and 0, 128 columns.)
-// 64 heads of 2048 x 1500 x 128: 408 us, bf16 without it 372.
+// 64 heads of 2048 x 1500 x 128: the pass takes 411 us, in bf16, without this, 368.
 struct Lift {
   int e = 126;               // nothing seen: values below 2^-111 pass as they are
   float up = 0x1p126f;       // 2^e

@@ -413,6 +413,8 @@ def cross_attention(q, k, v, kv_lengths=None, *, scale=None, return_lse=False, o
     float32, bfloat16 or float16; any strides with a contiguous last dimension.
     kv_lengths int32 [batch] (None: kv_len everywhere), held to [0, kv_len].
     scale defaults to 1 / sqrt(head_dim).  A row without keys gives zeros.
+    16-bit types: the softmax runs in fp32, its probabilities are rounded to the
+    type for the product with v.
     out, if given, receives the result; it must not share memory with k or v.
     Returns out like q, with return_lse also the log of each row's sum of
     exponentials, float32 [batch, heads, q_len] (-inf without keys).  No autograd
@@ -436,7 +438,9 @@ def cross_attention_backward(dout, q, k, v, out, lse, kv_lengths=None, *, scale=
     """Gradients (dq, dk, dv) of cross_attention for the gradient dout of its
     result.  out and lse are what cross_attention(..., return_lse=True) returned
     for the same q, k, v, kv_lengths and scale.  dk and dv are sums over the
-    query heads that share a head, and zero past a row's length.
+    query heads that share a head, and zero past a row's length.  16-bit types:
+    P and dS are rounded to the type for the products with dout, k and q (fp16
+    scaled by powers of two, so that values of any size keep their precision).
     """
     call = _call_of(q)
     q, k, v, (cfg, _, nbytes) = _xattn_inputs(call, q, k, v, scale)
