@@ -534,7 +534,8 @@ lcError_t lcCrossAttentionForward(const lcCrossAttentionConfig* cfg, const lcDev
  * types the second products take P (for dv) and dS = P o (dP - delta) (for dq and
  * dk) rounded to that type; fp16 holds both at powers of two, dS at one for each
  * query row and key, so that results inside fp16 keep its precision whatever the
- * size of dout and v and the number of keys (P below 2^-29 counts less exactly).
+ * size of dout and v and the number of keys (P below 2^-29, and dS below 2^-21 of
+ * the largest of its query row or key, count less exactly).
  * delta is the sum of P dP over a row's keys up to 128 of them, and of dout out,
  * with `out` as it was rounded, beyond. */
 lcError_t lcCrossAttentionBackward(const lcCrossAttentionConfig* cfg, const lcDeviceTensor* dout,

@@ -85,7 +85,7 @@ Status takeTensor(const char* op, const char* name, const lcDeviceTensor* t, std
         return fail(Status::kInvalidValue, who + " is written and has overlapping rows");
       }
       // No product of a stride that a real tensor can have overflows.
-      if (x.stride > (std::int64_t{1} << 62) / static_cast<std::int64_t>(x.n)) {
+      if (x.stride > (std::int64_t{1} << 60) / static_cast<std::int64_t>(x.n)) {
         return fail(Status::kNotSupported, who + " has a stride too large");
       }
       extent += x.stride * static_cast<std::int64_t>(x.n - 1);

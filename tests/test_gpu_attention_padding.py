@@ -56,3 +56,31 @@ def test_padding_changes_nothing(lc, dtype, d, sq):
             # border between two of its type's numbers falls on either side
             off = (x.double() - y.double()).norm() / y.double().norm().clamp_min(1e-30)
             assert off < U[dtype] / 4, (name, off)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_lengths_that_change_between_replays(lc, dtype):
+    """A captured pass takes delta by the lengths of the replay, on either side of 128."""
+    gen = torch.Generator()
+    gen.manual_seed(9)
+    q, dout = (torch.randn((3, 4, 40, 64), generator=gen).to(dtype).cuda() for _ in range(2))
+    k, v = (torch.randn((3, 2, 500, 64), generator=gen).to(dtype).cuda() for _ in range(2))
+    lengths = torch.tensor([500, 500, 500], dtype=torch.int32, device="cuda")
+
+    def run():
+        out, lse = lc.cross_attention(q, k, v, lengths, return_lse=True)
+        return (out, lse) + tuple(lc.cross_attention_backward(dout, q, k, v, out, lse, lengths))
+
+    run()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = run()
+    for turn in ([128, 129, 0], [1, 500, 127], [130, 2, 128], [500, 500, 500], [0, 0, 0]):
+        lengths.copy_(torch.tensor(turn))
+        graph.replay()
+        want = run()
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(got, want)), turn
+        ref = Attention(q, k, v, lengths).backward(dout)
+        for name, x in zip(("dq", "dk", "dv"), got[2:]):
+            assert_within(x, *ref[name], f"{turn} {name}")
